@@ -224,8 +224,83 @@ mgt_status_t mgt_launch_adamw(const mgt_adamw_config_t* config, float* device_we
 mgt_status_t mgt_launch_adamw_with_half_mirror(const mgt_adamw_config_t* config, float* device_weights,
                                                uint16_t* device_weights_half, const float* device_grad,
                                                float* device_m, float* device_v, void* stream);
+/* The same update of a gradient scaled by device_clip[1] (rounded to fp32), where mgt_launch_gradient_norm left {norm, scale} in device_clip: the gradient
+ * itself stays as it is. A scale of 1 gives the plain update bit for bit. Where the norm is not finite, weights, mirror and moments stay as
+ * they are. device_weights_half may be NULL (no mirror). No counterpart in the reference. */
+mgt_status_t mgt_launch_adamw_with_clip(const mgt_adamw_config_t* config, float* device_weights, uint16_t* device_weights_half, const float* device_grad,
+                                        const float* device_clip, float* device_m, float* device_v, void* stream);
 /* Replaces FloatToHalfMirrorKernel (native/tools/mgt_native_train_smoke.cu:68-72). */
 mgt_status_t mgt_launch_float_to_half(const float* device_values, uint64_t count, uint16_t* device_half, void* stream);
+
+/* ---- layer normalisation ---------------------------------------------------------------------
+ * Over the columns of every row of a [rows][cols] matrix; no counterpart in the reference (its networks have no normalisation,
+ * native/tools/mgt_native_train_smoke.cu:343). With mean and variance (biased) of a row and rstd = 1 / sqrt(variance + eps):
+ *   forward   y = gamma * (x - mean) * rstd + beta
+ *   backward  xhat = (x - mean) * rstd, g = dy * gamma, dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),
+ *             dgamma = sum over rows of dy * xhat, dbeta = of dy, dbias = of dx (the gradient of a bias vector that was added to
+ *             every row of x)
+ * Statistics and sums are fp32, dx enters dbias before it is rounded; results do not depend on the run (fixed orders of addition).
+ *   x_type, y_type, dx_type  types of x, of y and dy, and of dx. A 16-bit x goes with y and dy of its own type or fp32; dx has the
+ *                            type of x, or any where x and dy are fp32.
+ *   x_pitch, y_pitch, dx_pitch  elements from row to row (0 = cols) of x, of y and dy, and of dx; not less than cols. Elements between
+ *                            cols and the pitch are neither read nor written.
+ * cols 1 to MGT_LAYER_NORM_MAX_COLS; rows may be 0: nothing is read then, and the three sums are set to zero. Any alignment of whole
+ * elements will do; rows that begin on 16 bytes (8 beside an fp32 operand for a 16-bit one) are moved in wider accesses. y may be x, and dx
+ * may be dy or x, where type and pitch are the same; otherwise nothing overlaps. gamma NULL = ones, beta NULL = zeros;
+ * mean and rstd (rows floats, the forward pass leaves them for the backward pass) may be NULL in the forward pass; dgamma, dbeta and
+ * dbias may each be NULL (not wanted). gamma, beta and their gradients are fp32. A row with an infinity or a NaN gives NaN
+ * in that row (and, in the backward pass, in the sums). Deviations from the mean are squared in fp32: up to 1e18.
+ * The backward pass needs a workspace of mgt_layer_norm_backward_workspace_floats floats, 8-byte aligned (0 = invalid config); calls that may run at
+ * the same time need one each. Everything lies on the current device. */
+enum { MGT_F32 = 0, MGT_F16 = 1, MGT_BF16 = 2 };
+#define MGT_LAYER_NORM_MAX_COLS (1u << 20)
+typedef struct {
+    uint32_t rows;
+    uint32_t cols;
+    float eps; /* > 0, finite */
+    int32_t x_type;
+    int32_t y_type;
+    int32_t dx_type;
+    uint64_t x_pitch;
+    uint64_t y_pitch;
+    uint64_t dx_pitch;
+} mgt_layer_norm_config_t;
+
+mgt_status_t mgt_validate_layer_norm_config(const mgt_layer_norm_config_t* config);
+mgt_status_t mgt_launch_layer_norm(const mgt_layer_norm_config_t* config, const void* device_x, const float* device_gamma, const float* device_beta,
+                                   void* device_y, float* device_mean, float* device_rstd, void* stream);
+uint64_t mgt_layer_norm_backward_workspace_floats(const mgt_layer_norm_config_t* config);
+mgt_status_t mgt_launch_layer_norm_backward(const mgt_layer_norm_config_t* config, const void* device_dy, const void* device_x, const float* device_gamma,
+                                            const float* device_mean, const float* device_rstd, void* device_dx, float* device_dgamma, float* device_dbeta,
+                                            float* device_dbias, float* workspace, uint64_t workspace_floats, void* stream);
+
+/* ---- gradient norm and clipping -----------------------------------------------------------------
+ * The Euclidean norm of all elements of a list of tensors, the norm of each, and the factor that brings the whole to max_norm at
+ * most; no counterpart in the reference. Squares and sums are 64-bit, in an order that the list's sizes fix.
+ *   device_result        2 floats: norm, and scale = 1 where norm <= max_norm, max_norm / norm beyond, 0 where the norm is not a finite
+ *                        float (a NaN or an infinity in a gradient, or a norm beyond the largest float)
+ *   device_tensor_norms  tensor_count floats, may be NULL
+ *   max_norm             > 0; +infinity only measures
+ * A tensor is `count` elements side by side at `data` (any alignment of whole elements; count 0 is an empty tensor, whose norm is 0). The list is
+ * read during the call and may then go; 1 to MGT_MAX_TENSORS tensors of MGT_MAX_TENSOR_ELEMENTS elements together. The workspace
+ * (mgt_gradient_norm_workspace_floats floats, 8-byte aligned; 0 = invalid list) belongs to one call at a time.
+ * mgt_launch_clip_gradients multiplies every element by the scale that device_result holds, in fp32, rounded once, in place or (out_tensors
+ * not NULL: the same counts and types, not overlapping the list) to another place; a gradient whose norm is not finite becomes zero.
+ * Everything lies on the current device. */
+#define MGT_MAX_TENSORS 1024u
+#define MGT_MAX_TENSOR_ELEMENTS (1ull << 40)
+typedef struct {
+    void* data;
+    uint64_t count;
+    int32_t type; /* MGT_F32, MGT_F16 or MGT_BF16 */
+    int32_t reserved;
+} mgt_tensor_t;
+
+uint64_t mgt_gradient_norm_workspace_floats(const mgt_tensor_t* tensors, uint32_t tensor_count);
+mgt_status_t mgt_launch_gradient_norm(const mgt_tensor_t* tensors, uint32_t tensor_count, float max_norm, float* device_result,
+                                      float* device_tensor_norms, float* workspace, uint64_t workspace_floats, void* stream);
+mgt_status_t mgt_launch_clip_gradients(const mgt_tensor_t* tensors, uint32_t tensor_count, const float* device_result, const mgt_tensor_t* out_tensors,
+                                       void* stream);
 
 /* ---- gradient exchange between data-parallel ranks --------------------------------------------
  * Replaces the reference's NCCL wrapper (native/cuda/mgt_cuda/allreduce_nccl.cuh:14-24,

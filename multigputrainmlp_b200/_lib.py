@@ -51,6 +51,16 @@ def _declare(lib: C.CDLL) -> None:
     lib.mgt_validate_adamw_config.argtypes = [vp]
     lib.mgt_launch_adamw.argtypes = [vp, vp, vp, vp, vp, vp]
     lib.mgt_launch_adamw_with_half_mirror.argtypes = [vp, vp, vp, vp, vp, vp, vp]
+    lib.mgt_launch_adamw_with_clip.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mgt_validate_layer_norm_config.argtypes = [vp]
+    lib.mgt_launch_layer_norm.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mgt_layer_norm_backward_workspace_floats.restype = u64
+    lib.mgt_layer_norm_backward_workspace_floats.argtypes = [vp]
+    lib.mgt_launch_layer_norm_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, u64, vp]
+    lib.mgt_gradient_norm_workspace_floats.restype = u64
+    lib.mgt_gradient_norm_workspace_floats.argtypes = [vp, u32]
+    lib.mgt_launch_gradient_norm.argtypes = [vp, u32, f32, vp, vp, vp, u64, vp]
+    lib.mgt_launch_clip_gradients.argtypes = [vp, u32, vp, vp, vp]
     lib.mgt_launch_float_to_half.argtypes = [vp, u64, vp, vp]
     lib.mgt_debug_sums.argtypes = [vp, vp, u32, u32, u32, i32, vp, vp]
     lib.mgt_debug_gemm.argtypes = [vp, vp, u32, i32, vp, u32, i32, vp, u32, u32, u32, u32, vp, vp]

@@ -42,6 +42,29 @@ def _stream(stream):
     return C.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream))
 
 
+# element types of the operators that take more than one (MGT_F32, MGT_F16, MGT_BF16)
+F32, F16, BF16 = 0, 1, 2
+
+
+def _type_of(t):
+    """The type code of a torch tensor, None for any other type."""
+    import torch
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+
+
+def _unfit(t, type_code, elements) -> bool:
+    """Whether a tensor cannot stand for `elements` of a type from its address on: another type, another device than the current one
+    (the host included), or too little behind the address. None and plain addresses are the library's to judge."""
+    if t is None or not hasattr(t, "data_ptr"):
+        return False
+    import torch
+    if _type_of(t) != type_code or t.get_device() != torch.cuda.current_device():
+        return True
+    if t.is_contiguous():
+        return t.numel() < elements
+    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < elements
+
+
 class _WalkCfg(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("sample_count", "k_min", "k_max", "move_count", "state_len", "state_storage_len")]
 
@@ -53,6 +76,17 @@ class _Shape(C.Structure):
 class _Adam(C.Structure):
     _fields_ = [("param_count", C.c_uint64), ("step", C.c_uint64), ("learning_rate", C.c_float), ("beta1", C.c_float),
                 ("beta2", C.c_float), ("eps", C.c_float), ("weight_decay", C.c_float)]
+
+
+class _LayerNorm(C.Structure):
+    """mgt_layer_norm_config_t"""
+    _fields_ = [("rows", C.c_uint32), ("cols", C.c_uint32), ("eps", C.c_float), ("x_type", C.c_int32), ("y_type", C.c_int32), ("dx_type", C.c_int32),
+                ("x_pitch", C.c_uint64), ("y_pitch", C.c_uint64), ("dx_pitch", C.c_uint64)]
+
+
+class _Tensor(C.Structure):
+    """mgt_tensor_t"""
+    _fields_ = [("data", C.c_void_p), ("count", C.c_uint64), ("type", C.c_int32), ("reserved", C.c_int32)]
 
 
 class BackwardProfile(C.Structure):
@@ -293,3 +327,115 @@ def launch_adamw_kernel_with_half_mirror(config, device_weights, device_weights_
 
 def launch_float_to_half(device_values, count, device_half, stream=None) -> int:
     return int(_lib.load().mgt_launch_float_to_half(_ptr(device_values), count, _ptr(device_half), _stream(stream)))
+
+
+def launch_adamw_kernel_with_clip(config, device_weights, device_weights_half, device_grad, device_clip, device_m, device_v, stream=None) -> int:
+    """mgt_launch_adamw_with_clip: the update of a gradient scaled by device_clip[1], skipped where the norm device_clip[0] is not finite
+    (what launch_gradient_norm leaves). device_weights_half may be None."""
+    n = config.param_count
+    if any(_unfit(t, F32, n) for t in (device_weights, device_grad, device_m, device_v)) or _unfit(device_weights_half, F16, n) or _unfit(device_clip, F32, 2):
+        return 1
+    cfg = config.c()
+    return int(_lib.load().mgt_launch_adamw_with_clip(C.byref(cfg), _ptr(device_weights), _ptr(device_weights_half), _ptr(device_grad),
+                                                      _ptr(device_clip), _ptr(device_m), _ptr(device_v), _stream(stream)))
+
+
+@dataclass
+class LayerNormConfig:
+    """mgt_layer_norm_config_t. y_type and y_pitch are those of dy in the backward pass; dx_type None = x_type; a pitch of 0 = cols."""
+    rows: int
+    cols: int
+    eps: float = 1e-5
+    x_type: int = F32
+    y_type: int = F32
+    dx_type: int | None = None
+    x_pitch: int = 0
+    y_pitch: int = 0
+    dx_pitch: int = 0
+
+    def c(self):
+        if not 0 <= self.rows < 2**32 or not 0 <= self.cols < 2**32 or min(self.x_pitch, self.y_pitch, self.dx_pitch) < 0:
+            return _LayerNorm()  # (no columns: refused; the fields would wrap)
+        return _LayerNorm(self.rows, self.cols, self.eps, self.x_type, self.y_type, self.x_type if self.dx_type is None else self.dx_type,
+                          self.x_pitch, self.y_pitch, self.dx_pitch)
+
+    def _extent(self, pitch: int) -> int:
+        return (self.rows - 1) * (pitch or self.cols) + self.cols if self.rows else 0
+
+
+def validate_layer_norm_config(config: LayerNormConfig) -> int:
+    cfg = config.c()
+    return int(_lib.load().mgt_validate_layer_norm_config(C.byref(cfg)))
+
+
+def launch_layer_norm(config: LayerNormConfig, x, gamma, beta, y, mean=None, rstd=None, stream=None) -> int:
+    """mgt_launch_layer_norm: y = gamma * (x - mean) * rstd + beta over the columns of every row; gamma, beta, mean and rstd may be None.
+    A tensor of another type, on another device than the current one, or too small, is refused (1)."""
+    if (_unfit(x, config.x_type, config._extent(config.x_pitch)) or _unfit(y, config.y_type, config._extent(config.y_pitch))
+            or any(_unfit(t, F32, config.cols) for t in (gamma, beta)) or any(_unfit(t, F32, config.rows) for t in (mean, rstd))):
+        return 1
+    cfg = config.c()
+    return int(_lib.load().mgt_launch_layer_norm(C.byref(cfg), _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), _stream(stream)))
+
+
+def layer_norm_backward_workspace_floats(config: LayerNormConfig) -> int:
+    cfg = config.c()
+    return int(_lib.load().mgt_layer_norm_backward_workspace_floats(C.byref(cfg)))
+
+
+def launch_layer_norm_backward(config: LayerNormConfig, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, dbias, workspace, workspace_floats, stream=None) -> int:
+    """mgt_launch_layer_norm_backward: dx, and the sums over the rows dgamma, dbeta and dbias (each may be None)."""
+    if (_unfit(dy, config.y_type, config._extent(config.y_pitch)) or _unfit(x, config.x_type, config._extent(config.x_pitch))
+            or _unfit(dx, config.x_type if config.dx_type is None else config.dx_type, config._extent(config.dx_pitch))
+            or any(_unfit(t, F32, config.cols) for t in (gamma, dgamma, dbeta, dbias)) or any(_unfit(t, F32, config.rows) for t in (mean, rstd))
+            or _unfit(workspace, F32, workspace_floats)):
+        return 1
+    cfg = config.c()
+    return int(_lib.load().mgt_launch_layer_norm_backward(C.byref(cfg), _ptr(dy), _ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dgamma),
+                                                          _ptr(dbeta), _ptr(dbias), _ptr(workspace), workspace_floats, _stream(stream)))
+
+
+class TensorList:
+    """An array of mgt_tensor_t for the gradient-norm calls, and the tensors it stands for: float32, float16 or bfloat16, each dense,
+    all on one CUDA device. Built once where gradients stay in place; holds the tensors, not their values."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.count = len(self.tensors)
+        self._array = (_Tensor * max(1, self.count))()
+        devices = set()
+        for entry, t in zip(self._array, self.tensors):
+            kind = _type_of(t)
+            if kind is None or not t.is_contiguous() or not t.is_cuda:
+                raise MgtError(1, "TensorList: dense CUDA tensors of float32, float16 or bfloat16")
+            entry.data, entry.count, entry.type = t.data_ptr(), t.numel(), kind
+            devices.add(t.get_device())
+        if len(devices) != 1:
+            raise MgtError(1, "TensorList: tensors of one device")
+        self.device = devices.pop()
+        self.pointer = C.cast(self._array, C.c_void_p)
+
+
+def _elsewhere(tensors: TensorList) -> bool:
+    import torch
+    return tensors.device != torch.cuda.current_device()
+
+
+def gradient_norm_workspace_floats(tensors: TensorList) -> int:
+    return int(_lib.load().mgt_gradient_norm_workspace_floats(tensors.pointer, tensors.count))
+
+
+def launch_gradient_norm(tensors: TensorList, max_norm: float, result, tensor_norms, workspace, workspace_floats, stream=None) -> int:
+    """mgt_launch_gradient_norm: result = {norm over all tensors, scale that brings it to max_norm at most}; tensor_norms (may be None) = the norm of each."""
+    if _elsewhere(tensors) or _unfit(result, F32, 2) or _unfit(tensor_norms, F32, tensors.count) or _unfit(workspace, F32, workspace_floats):
+        return 1
+    return int(_lib.load().mgt_launch_gradient_norm(tensors.pointer, tensors.count, max_norm, _ptr(result), _ptr(tensor_norms), _ptr(workspace),
+                                                    workspace_floats, _stream(stream)))
+
+
+def launch_clip_gradients(tensors: TensorList, result, out_tensors: TensorList | None = None, stream=None) -> int:
+    """mgt_launch_clip_gradients: every element times result[1], in place or into out_tensors (same counts and types)."""
+    if _elsewhere(tensors) or _unfit(result, F32, 2) or (out_tensors is not None and (_elsewhere(out_tensors) or out_tensors.count != tensors.count)):
+        return 1
+    return int(_lib.load().mgt_launch_clip_gradients(tensors.pointer, tensors.count, _ptr(result), out_tensors.pointer if out_tensors is not None else None,
+                                                     _stream(stream)))

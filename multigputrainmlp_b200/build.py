@@ -22,7 +22,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr",
 ]
-CUDA_SOURCES = ["walk.cu", "adamw.cu", "engine.cu", "comm.cu"]
+CUDA_SOURCES = ["walk.cu", "adamw.cu", "engine.cu", "comm.cu", "layer_norm_forward.cu", "layer_norm_backward.cu", "gradient_clip.cu"]
 HOST_SOURCES = ["plan.cpp", "artifacts.cpp", "host_capi.cpp"]
 
 

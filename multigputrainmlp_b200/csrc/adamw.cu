@@ -12,19 +12,27 @@ namespace {
 constexpr uint32_t kAdamWThreads = 128;
 constexpr uint64_t kOverlapParams = 8ULL << 20;  // a longer update does not notice the gap before it, and its CTAs crowd what still runs
 
-template <bool kMirror>
+// kClip: the gradient is scaled by clip[1] on its way, and a norm clip[0] that is not finite leaves everything as it is.
+template <bool kMirror, bool kClip>
 __global__ void __launch_bounds__(kAdamWThreads)
 AdamWKernel(mgt_adamw_config_t config, float* __restrict__ w, __half* __restrict__ w_half, const float* __restrict__ g,
-            float* __restrict__ m, float* __restrict__ v) {
+            float* __restrict__ m, float* __restrict__ v, const float* __restrict__ clip) {
     const mgt::AdamWScalars sc = mgt::MakeAdamWScalars(config.step, config.learning_rate, config.beta1, config.beta2, config.eps, config.weight_decay);
     const uint64_t n4 = config.param_count >> 2;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
     mgt::dependent_begin();
+    float scale = 1.0f;
+    if (kClip) {
+        const float* c = mgt::after_begin(clip);
+        if (!(c[0] <= 3.402823466e38f)) return;
+        scale = c[1];
+    }
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n4; i += stride) {
         float4 wv = reinterpret_cast<float4*>(w)[i];
-        const float4 gv = reinterpret_cast<const float4*>(g)[i];
+        float4 gv = reinterpret_cast<const float4*>(g)[i];
         float4 mv = reinterpret_cast<float4*>(m)[i];
         float4 vv = reinterpret_cast<float4*>(v)[i];
+        if (kClip) gv = make_float4(__fmul_rn(gv.x, scale), __fmul_rn(gv.y, scale), __fmul_rn(gv.z, scale), __fmul_rn(gv.w, scale));
         wv.x = mgt::AdamWUpdateOne(sc, wv.x, gv.x, &mv.x, &vv.x);
         wv.y = mgt::AdamWUpdateOne(sc, wv.y, gv.y, &mv.y, &vv.y);
         wv.z = mgt::AdamWUpdateOne(sc, wv.z, gv.z, &mv.z, &vv.z);
@@ -46,7 +54,7 @@ AdamWKernel(mgt_adamw_config_t config, float* __restrict__ w, __half* __restrict
     const uint64_t t = tail0 + static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (t < config.param_count) {
         float mm = m[t], vv = v[t];
-        const float nw = mgt::AdamWUpdateOne(sc, w[t], g[t], &mm, &vv);
+        const float nw = mgt::AdamWUpdateOne(sc, w[t], kClip ? __fmul_rn(g[t], scale) : g[t], &mm, &vv);
         w[t] = nw;
         m[t] = mm;
         v[t] = vv;
@@ -82,7 +90,7 @@ mgt_status_t mgt_validate_adamw_config(const mgt_adamw_config_t* c) {
 }
 
 static mgt_status_t LaunchAdamW(const mgt_adamw_config_t* config, float* w, uint16_t* w_half, const float* g, float* m, float* v,
-                                void* stream, bool mirror) {
+                                void* stream, bool mirror, const float* clip = nullptr) {
     if (mgt_validate_adamw_config(config) != MGT_OK || w == nullptr || g == nullptr || m == nullptr || v == nullptr ||
         (mirror && w_half == nullptr)) {
         return MGT_INVALID_CONFIG;
@@ -97,11 +105,8 @@ static mgt_status_t LaunchAdamW(const mgt_adamw_config_t* config, float* w, uint
     const uint64_t cap = 1ULL << 30;
     const uint32_t blocks = static_cast<uint32_t>(want < 1 ? 1 : (want < cap ? want : cap));
     const mgt::LaunchOn s(static_cast<cudaStream_t>(stream), config->param_count <= kOverlapParams);
-    if (mirror) {
-        mgt::Launch(AdamWKernel<true>, blocks, kAdamWThreads, 0, s, *config, w, reinterpret_cast<__half*>(w_half), g, m, v);
-    } else {
-        mgt::Launch(AdamWKernel<false>, blocks, kAdamWThreads, 0, s, *config, w, nullptr, g, m, v);
-    }
+    auto kernel = mirror ? (clip != nullptr ? AdamWKernel<true, true> : AdamWKernel<true, false>) : (clip != nullptr ? AdamWKernel<false, true> : AdamWKernel<false, false>);
+    mgt::Launch(kernel, blocks, kAdamWThreads, 0, s, *config, w, reinterpret_cast<__half*>(w_half), g, m, v, clip);
     return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
 }
 
@@ -112,6 +117,12 @@ mgt_status_t mgt_launch_adamw(const mgt_adamw_config_t* config, float* w, const 
 mgt_status_t mgt_launch_adamw_with_half_mirror(const mgt_adamw_config_t* config, float* w, uint16_t* w_half, const float* g,
                                                float* m, float* v, void* stream) {
     return LaunchAdamW(config, w, w_half, g, m, v, stream, true);
+}
+
+mgt_status_t mgt_launch_adamw_with_clip(const mgt_adamw_config_t* config, float* w, uint16_t* w_half, const float* g, const float* clip,
+                                        float* m, float* v, void* stream) {
+    if (clip == nullptr || (reinterpret_cast<uintptr_t>(clip) & 3U) != 0) return MGT_INVALID_CONFIG;
+    return LaunchAdamW(config, w, w_half, g, m, v, stream, w_half != nullptr, clip);
 }
 
 mgt_status_t mgt_launch_float_to_half(const float* values, uint64_t count, uint16_t* half, void* stream) {
