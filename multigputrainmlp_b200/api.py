@@ -46,23 +46,46 @@ def _stream(stream):
 F32, F16, BF16 = 0, 1, 2
 
 
-def _type_of(t):
-    """The type code of a torch tensor, None for any other type."""
-    import torch
-    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+_torch = None
 
 
-def _unfit(t, type_code, elements) -> bool:
-    """Whether a tensor cannot stand for `elements` of a type from its address on: another type, another device than the current one
-    (the host included), or too little behind the address. None and plain addresses are the library's to judge."""
+def _with_torch():
+    global _torch, _TYPES
+    if _torch is None:
+        import torch
+        _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        _torch = torch
+    return _torch
+
+
+def _unfit(t, type_code, elements, device) -> bool:
+    """Whether a tensor cannot stand for `elements` of a type from its address on: another type, another device than `device` (the host
+    included), or too little behind the address. None and plain addresses are the library's to judge."""
     if t is None or not hasattr(t, "data_ptr"):
         return False
-    import torch
-    if _type_of(t) != type_code or t.get_device() != torch.cuda.current_device():
+    if _TYPES.get(t.dtype) != type_code or t.get_device() != device:
         return True
     if t.is_contiguous():
         return t.numel() < elements
     return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < elements
+
+
+def _at(t):
+    """The address behind a tensor, or the address itself."""
+    return t.data_ptr() if hasattr(t, "data_ptr") else t
+
+
+def _raw_stream(stream, device):
+    """The cudaStream_t of a stream, of the current one where there is none (without building an object for it: 1.5 us)."""
+    if stream is None:
+        return _torch._C._cuda_getCurrentRawStream(device)
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _current_device(stream):
+    """The current device, of which tensors have to be. With plain addresses and a stream nothing is asked of torch's CUDA side."""
+    torch = _with_torch()
+    return torch.cuda.current_device() if stream is None or torch.cuda.is_initialized() else None
 
 
 class _WalkCfg(C.Structure):
@@ -332,15 +355,16 @@ def launch_float_to_half(device_values, count, device_half, stream=None) -> int:
 def launch_adamw_kernel_with_clip(config, device_weights, device_weights_half, device_grad, device_clip, device_m, device_v, stream=None) -> int:
     """mgt_launch_adamw_with_clip: the update of a gradient scaled by device_clip[1], skipped where the norm device_clip[0] is not finite
     (what launch_gradient_norm leaves). device_weights_half may be None."""
-    n = config.param_count
-    if any(_unfit(t, F32, n) for t in (device_weights, device_grad, device_m, device_v)) or _unfit(device_weights_half, F16, n) or _unfit(device_clip, F32, 2):
+    n, d = config.param_count, _current_device(stream)
+    if (_unfit(device_weights, F32, n, d) or _unfit(device_grad, F32, n, d) or _unfit(device_m, F32, n, d) or _unfit(device_v, F32, n, d)
+            or _unfit(device_weights_half, F16, n, d) or _unfit(device_clip, F32, 2, d)):
         return 1
     cfg = config.c()
-    return int(_lib.load().mgt_launch_adamw_with_clip(C.byref(cfg), _ptr(device_weights), _ptr(device_weights_half), _ptr(device_grad),
-                                                      _ptr(device_clip), _ptr(device_m), _ptr(device_v), _stream(stream)))
+    return _lib.load().mgt_launch_adamw_with_clip(C.byref(cfg), _at(device_weights), _at(device_weights_half), _at(device_grad), _at(device_clip),
+                                                  _at(device_m), _at(device_v), _raw_stream(stream, d))
 
 
-@dataclass
+@dataclass(frozen=True)
 class LayerNormConfig:
     """mgt_layer_norm_config_t. y_type and y_pitch are those of dy in the backward pass; dx_type None = x_type; a pitch of 0 = cols."""
     rows: int
@@ -353,46 +377,48 @@ class LayerNormConfig:
     y_pitch: int = 0
     dx_pitch: int = 0
 
-    def c(self):
-        if not 0 <= self.rows < 2**32 or not 0 <= self.cols < 2**32 or min(self.x_pitch, self.y_pitch, self.dx_pitch) < 0:
-            return _LayerNorm()  # (no columns: refused; the fields would wrap)
-        return _LayerNorm(self.rows, self.cols, self.eps, self.x_type, self.y_type, self.x_type if self.dx_type is None else self.dx_type,
-                          self.x_pitch, self.y_pitch, self.dx_pitch)
+    def __post_init__(self):
+        fits = 0 <= self.rows < 2**32 and 0 <= self.cols < 2**32 and min(self.x_pitch, self.y_pitch, self.dx_pitch) >= 0
+        dx_type = self.x_type if self.dx_type is None else self.dx_type
+        # (what a field would wrap around is refused as a config without columns)
+        c = _LayerNorm(self.rows, self.cols, self.eps, self.x_type, self.y_type, dx_type, self.x_pitch, self.y_pitch, self.dx_pitch) if fits else _LayerNorm()
+        extents = tuple((self.rows - 1) * (pitch or self.cols) + self.cols if self.rows else 0 for pitch in (self.x_pitch, self.y_pitch, self.dx_pitch))
+        for name, value in (("_c", c), ("_reference", C.byref(c)), ("_extents", extents), ("_dx_type", dx_type)):
+            object.__setattr__(self, name, value)
 
-    def _extent(self, pitch: int) -> int:
-        return (self.rows - 1) * (pitch or self.cols) + self.cols if self.rows else 0
+    def c(self):
+        return self._c
 
 
 def validate_layer_norm_config(config: LayerNormConfig) -> int:
-    cfg = config.c()
-    return int(_lib.load().mgt_validate_layer_norm_config(C.byref(cfg)))
+    return _lib.load().mgt_validate_layer_norm_config(config._reference)
 
 
 def launch_layer_norm(config: LayerNormConfig, x, gamma, beta, y, mean=None, rstd=None, stream=None) -> int:
     """mgt_launch_layer_norm: y = gamma * (x - mean) * rstd + beta over the columns of every row; gamma, beta, mean and rstd may be None.
     A tensor of another type, on another device than the current one, or too small, is refused (1)."""
-    if (_unfit(x, config.x_type, config._extent(config.x_pitch)) or _unfit(y, config.y_type, config._extent(config.y_pitch))
-            or any(_unfit(t, F32, config.cols) for t in (gamma, beta)) or any(_unfit(t, F32, config.rows) for t in (mean, rstd))):
+    d = _current_device(stream)
+    x_extent, y_extent, _ = config._extents
+    if (_unfit(x, config.x_type, x_extent, d) or _unfit(y, config.y_type, y_extent, d) or _unfit(gamma, F32, config.cols, d) or _unfit(beta, F32, config.cols, d)
+            or _unfit(mean, F32, config.rows, d) or _unfit(rstd, F32, config.rows, d)):
         return 1
-    cfg = config.c()
-    return int(_lib.load().mgt_launch_layer_norm(C.byref(cfg), _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), _stream(stream)))
+    return _lib.load().mgt_launch_layer_norm(config._reference, _at(x), _at(gamma), _at(beta), _at(y), _at(mean), _at(rstd), _raw_stream(stream, d))
 
 
 def layer_norm_backward_workspace_floats(config: LayerNormConfig) -> int:
-    cfg = config.c()
-    return int(_lib.load().mgt_layer_norm_backward_workspace_floats(C.byref(cfg)))
+    return _lib.load().mgt_layer_norm_backward_workspace_floats(config._reference)
 
 
 def launch_layer_norm_backward(config: LayerNormConfig, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, dbias, workspace, workspace_floats, stream=None) -> int:
     """mgt_launch_layer_norm_backward: dx, and the sums over the rows dgamma, dbeta and dbias (each may be None)."""
-    if (_unfit(dy, config.y_type, config._extent(config.y_pitch)) or _unfit(x, config.x_type, config._extent(config.x_pitch))
-            or _unfit(dx, config.x_type if config.dx_type is None else config.dx_type, config._extent(config.dx_pitch))
-            or any(_unfit(t, F32, config.cols) for t in (gamma, dgamma, dbeta, dbias)) or any(_unfit(t, F32, config.rows) for t in (mean, rstd))
-            or _unfit(workspace, F32, workspace_floats)):
+    d = _current_device(stream)
+    x_extent, dy_extent, dx_extent = config._extents
+    if (_unfit(dy, config.y_type, dy_extent, d) or _unfit(x, config.x_type, x_extent, d) or _unfit(dx, config._dx_type, dx_extent, d)
+            or _unfit(gamma, F32, config.cols, d) or _unfit(dgamma, F32, config.cols, d) or _unfit(dbeta, F32, config.cols, d) or _unfit(dbias, F32, config.cols, d)
+            or _unfit(mean, F32, config.rows, d) or _unfit(rstd, F32, config.rows, d) or _unfit(workspace, F32, workspace_floats, d)):
         return 1
-    cfg = config.c()
-    return int(_lib.load().mgt_launch_layer_norm_backward(C.byref(cfg), _ptr(dy), _ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dgamma),
-                                                          _ptr(dbeta), _ptr(dbias), _ptr(workspace), workspace_floats, _stream(stream)))
+    return _lib.load().mgt_launch_layer_norm_backward(config._reference, _at(dy), _at(x), _at(gamma), _at(mean), _at(rstd), _at(dx), _at(dgamma), _at(dbeta),
+                                                      _at(dbias), _at(workspace), workspace_floats, _raw_stream(stream, d))
 
 
 class TensorList:
@@ -400,12 +426,13 @@ class TensorList:
     all on one CUDA device. Built once where gradients stay in place; holds the tensors, not their values."""
 
     def __init__(self, tensors):
+        _with_torch()
         self.tensors = list(tensors)
         self.count = len(self.tensors)
         self._array = (_Tensor * max(1, self.count))()
         devices = set()
         for entry, t in zip(self._array, self.tensors):
-            kind = _type_of(t)
+            kind = _TYPES.get(t.dtype)
             if kind is None or not t.is_contiguous() or not t.is_cuda:
                 raise MgtError(1, "TensorList: dense CUDA tensors of float32, float16 or bfloat16")
             entry.data, entry.count, entry.type = t.data_ptr(), t.numel(), kind
@@ -413,29 +440,26 @@ class TensorList:
         if len(devices) != 1:
             raise MgtError(1, "TensorList: tensors of one device")
         self.device = devices.pop()
-        self.pointer = C.cast(self._array, C.c_void_p)
-
-
-def _elsewhere(tensors: TensorList) -> bool:
-    import torch
-    return tensors.device != torch.cuda.current_device()
+        self.pointer = C.addressof(self._array)
 
 
 def gradient_norm_workspace_floats(tensors: TensorList) -> int:
-    return int(_lib.load().mgt_gradient_norm_workspace_floats(tensors.pointer, tensors.count))
+    return _lib.load().mgt_gradient_norm_workspace_floats(tensors.pointer, tensors.count)
 
 
 def launch_gradient_norm(tensors: TensorList, max_norm: float, result, tensor_norms, workspace, workspace_floats, stream=None) -> int:
     """mgt_launch_gradient_norm: result = {norm over all tensors, scale that brings it to max_norm at most}; tensor_norms (may be None) = the norm of each."""
-    if _elsewhere(tensors) or _unfit(result, F32, 2) or _unfit(tensor_norms, F32, tensors.count) or _unfit(workspace, F32, workspace_floats):
+    d = _current_device(stream)
+    if tensors.device != d or _unfit(result, F32, 2, d) or _unfit(tensor_norms, F32, tensors.count, d) or _unfit(workspace, F32, workspace_floats, d):
         return 1
-    return int(_lib.load().mgt_launch_gradient_norm(tensors.pointer, tensors.count, max_norm, _ptr(result), _ptr(tensor_norms), _ptr(workspace),
-                                                    workspace_floats, _stream(stream)))
+    return _lib.load().mgt_launch_gradient_norm(tensors.pointer, tensors.count, max_norm, _at(result), _at(tensor_norms), _at(workspace), workspace_floats,
+                                                _raw_stream(stream, d))
 
 
 def launch_clip_gradients(tensors: TensorList, result, out_tensors: TensorList | None = None, stream=None) -> int:
     """mgt_launch_clip_gradients: every element times result[1], in place or into out_tensors (same counts and types)."""
-    if _elsewhere(tensors) or _unfit(result, F32, 2) or (out_tensors is not None and (_elsewhere(out_tensors) or out_tensors.count != tensors.count)):
+    d = _current_device(stream)
+    if tensors.device != d or _unfit(result, F32, 2, d) or (out_tensors is not None and (out_tensors.device != d or out_tensors.count != tensors.count)):
         return 1
-    return int(_lib.load().mgt_launch_clip_gradients(tensors.pointer, tensors.count, _ptr(result), out_tensors.pointer if out_tensors is not None else None,
-                                                     _stream(stream)))
+    return _lib.load().mgt_launch_clip_gradients(tensors.pointer, tensors.count, _at(result), out_tensors.pointer if out_tensors is not None else None,
+                                                 _raw_stream(stream, d))

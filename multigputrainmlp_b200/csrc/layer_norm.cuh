@@ -1,12 +1,18 @@
-// Layer normalisation: how a row is held. A row of C columns is shared by `lanes` threads (a power of two, at most a CTA); thread t has
-// the packs t, t + lanes, ... of V neighbouring elements, NV of them at most, all in registers, so that a row is read once. Several rows
-// lie side by side in a CTA. Groups of up to 32 lanes reduce by shuffles, wider ones through shared memory and a barrier of their own.
+// Layer normalisation: how rows are held and fetched. A row of C columns is shared by `lanes` threads (a power of two, at most a CTA); thread
+// t has the packs t, t + lanes, ... of V neighbouring elements, at most 16 elements in all. Several rows lie side by side in a CTA. Groups
+// of up to 32 lanes reduce by shuffles, wider ones through shared memory and a barrier of their own.
+//
+// The kernels are bound by HBM, and what that takes is bytes in flight: some 45 KB an SM at 6.5 TB/s and a loaded latency of 1 us. One
+// row ahead in registers leaves 24 KB in flight (131 072 x 512 bf16 forward 107 us); so a thread copies what it will need of its next rows to
+// shared memory asynchronously, several rows deep.
 #pragma once
 
 #include "layer_norm.hpp"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 namespace mgt {
 namespace ln {
@@ -19,44 +25,54 @@ template <> __device__ __forceinline__ float FromFloat<float>(float v) { return 
 template <> __device__ __forceinline__ __half FromFloat<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V neighbouring elements as they lie in memory, moved in accesses of up to 16 bytes.
+// V neighbouring elements as they lie in memory, moved in one access.
 template <class T, int V>
-struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
+struct alignas(sizeof(T) * V) Pack {
     T v[V];
 };
 template <int kBytes> struct Word { using type = uint4; };
 template <> struct Word<8> { using type = uint2; };
 template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<2> { using type = uint16_t; };
-
 template <class T, int V>
-__device__ __forceinline__ void LoadPack(Pack<T, V>& out, const T* p, uint32_t valid) {
-    using W = typename Word<(sizeof(T) * V > 16 ? 16 : sizeof(T) * V)>::type;
-    constexpr int kWords = sizeof(T) * V / sizeof(W);
-    if (valid >= V) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) reinterpret_cast<W*>(&out)[i] = reinterpret_cast<const W*>(p)[i];
-    } else {  // the last pack of a row, or none of it
-#pragma unroll
-        for (int i = 0; i < V; ++i) out.v[i] = i < valid ? p[i] : FromFloat<T>(0.0f);
-    }
-}
-template <class T, int V>
-__device__ __forceinline__ void StorePack(T* p, const float (&v)[V], uint32_t valid) {
-    using W = typename Word<(sizeof(T) * V > 16 ? 16 : sizeof(T) * V)>::type;
-    constexpr int kWords = sizeof(T) * V / sizeof(W);
+__device__ __forceinline__ Pack<T, V> LoadPack(const T* p) {
     Pack<T, V> out;
-#pragma unroll
-    for (int i = 0; i < V; ++i) out.v[i] = FromFloat<T>(v[i]);
-    if (valid >= V) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) reinterpret_cast<W*>(p)[i] = reinterpret_cast<const W*>(&out)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < valid) p[i] = out.v[i];
-    }
+    using W = typename Word<sizeof(T) * V>::type;
+    *reinterpret_cast<W*>(&out) = *reinterpret_cast<const W*>(p);
+    return out;
 }
+template <class T, int V>
+__device__ __forceinline__ void StorePack(T* p, const Pack<T, V>& v) {
+    using W = typename Word<sizeof(T) * V>::type;
+    *reinterpret_cast<W*>(p) = *reinterpret_cast<const W*>(&v);
+}
+
+// The elements that a thread holds of a row, as fp32 pairs (one element alone has a zero beside it): half as many instructions as by
+// single values, and instructions are what bounds these kernels once their loads are far enough ahead.
+__device__ __forceinline__ uint64_t& Bits(float2& v) { return reinterpret_cast<uint64_t&>(v); }
+__device__ __forceinline__ float2 Add2(float2 a, float2 b) {
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(Bits(a)) : "l"(Bits(b)));
+    return a;
+}
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(Bits(a)) : "l"(Bits(b)));
+    return a;
+}
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(Bits(c)) : "l"(Bits(a)), "l"(Bits(b)));
+    return c;
+}
+__device__ __forceinline__ float2 Both(float v) { return make_float2(v, v); }
+template <int E>
+struct Held {
+    static constexpr int kPairs = (E + 1) / 2;
+    float2 pair[kPairs];
+    __device__ __forceinline__ void Set(int k, float v) {
+        if (k & 1) pair[k / 2].y = v; else pair[k / 2].x = v;
+        if (E == 1) pair[0].y = 0.0f;
+    }
+    __device__ __forceinline__ float Get(int k) const { return k & 1 ? pair[k / 2].y : pair[k / 2].x; }
+};
 
 // The threads that share a row. Reductions alternate between two buffers: who writes one again has passed the barrier of the other, and
 // with it everybody's reads of this one.
@@ -68,72 +84,211 @@ struct Group {
 __device__ __forceinline__ Group MakeGroup(uint32_t lanes, float2* buffer) {
     return {lanes, threadIdx.x & (lanes - 1U), threadIdx.x / lanes, blockDim.x / lanes, buffer, 0U};
 }
-// Sums of a and b over the group, in every one of its threads. All threads of a warp come here together.
-__device__ __forceinline__ float2 Reduce(Group& g, float a, float b) {
-    for (uint32_t o = min(g.lanes, 32U) >> 1; o > 0U; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffU, a, o);
-        b += __shfl_xor_sync(0xffffffffU, b, o);
+// Sums of one or two values over the group, in every one of its threads. All threads of a warp come here together.
+template <int N>
+__device__ __forceinline__ void Reduce(Group& g, float (&v)[N]) {
+#pragma unroll
+    for (uint32_t o = 16U; o > 0U; o >>= 1) {
+        if (o >= g.lanes) continue;  // (the same for the whole CTA)
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffU, v[n], o);
     }
     if (g.lanes > 32U) {
         const uint32_t warps = g.lanes >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31U;
         float2* at = g.buffer + (g.turn & 1U) * (blockDim.x >> 5);
         g.turn ^= 1U;
-        if (lane == 0U) at[warp] = make_float2(a, b);
+        if (lane == 0U) at[warp] = make_float2(v[0], v[N - 1]);
         asm volatile("bar.sync %0, %1;" ::"r"(1U + g.index), "r"(g.lanes) : "memory");
-        const float2 part = lane < warps ? at[g.index * warps + lane] : make_float2(0.0f, 0.0f);
-        a = part.x;
-        b = part.y;
-        for (uint32_t o = warps >> 1; o > 0U; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffU, a, o);
-            b += __shfl_xor_sync(0xffffffffU, b, o);
+        const float2 part = at[g.index * warps + (lane & (warps - 1U))];  // (each of them in 32 / warps lanes: no broadcast behind the tree)
+        v[0] = part.x;
+        v[N - 1] = N > 1 ? part.y : part.x;
+#pragma unroll
+        for (uint32_t o = 16U; o > 0U; o >>= 1) {
+            if (o >= warps) continue;
+#pragma unroll
+            for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffU, v[n], o);
         }
-        a = __shfl_sync(0xffffffffU, a, 0);
-        b = __shfl_sync(0xffffffffU, b, 0);
     }
-    return make_float2(a, b);
 }
 
-// Column of this thread's pack i, and how many of its elements the row has.
+// Which rows a group has: the first one, every stride-th from there, `mine` in all; `turns` of the warp's group that has most.
+struct Share {
+    uint32_t first, stride, mine, turns;
+};
+__device__ __forceinline__ Share MakeShare(const Group& g, uint32_t rows) {
+    Share s;
+    s.first = blockIdx.x * g.count + g.index;
+    s.stride = gridDim.x * g.count;
+    const uint32_t least = g.lanes < 32U ? s.first - (g.index & (32U / g.lanes - 1U)) : s.first;
+    s.mine = s.first < rows ? (rows - 1U - s.first) / s.stride + 1U : 0U;
+    s.turns = least < rows ? (rows - 1U - least) / s.stride + 1U : 0U;
+    return s;
+}
+
+// Column of this thread's pack i. Packs are whole: the row has all of one or nothing.
 template <int V>
 __device__ __forceinline__ uint32_t PackColumn(const Group& g, int i) { return (static_cast<uint32_t>(i) * g.lanes + g.lane) * V; }
-__device__ __forceinline__ uint32_t PackValid(uint32_t column, uint32_t cols) { return column < cols ? cols - column : 0U; }
+
+template <int kBytes>
+__device__ __forceinline__ void CopyAsync(uint32_t to, const void* from) {
+    if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void CopiesEnd() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void CopiesWait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// What a thread has of its next kDepth rows of one operand, in shared memory.
+//   V > 1   packs of 16 (or 8) bytes. A thread reads only what it copied itself: nothing is shared, and nothing waits.
+//   V = 1   rows that begin anywhere: the group copies the 16-byte lines that its row lies in, and a thread reads its elements from them
+//           behind a barrier of the group. Lines that reach beyond the matrix are copied by elements.
+template <class T, int V, int NV, int kThreads, int kDepth>
+struct Ring {
+    static constexpr uint32_t kPackBytes = sizeof(T) * V;
+    const T* next;       // the row to be fetched next
+    const T* now;        // the row to be read next
+    uint64_t step;       // elements from a row of the group to its next
+    uint32_t cols, line_bytes;  // line_bytes: of a group's row (V = 1)
+    char* slots;         // of this thread (V > 1) or group
+    uintptr_t least, most;      // the matrix (V = 1)
+
+    static __host__ __device__ uint32_t LineBytes(uint32_t cols) { return (cols * static_cast<uint32_t>(sizeof(T)) + 15U) / 16U * 16U + 16U; }
+    static __host__ __device__ uint32_t Bytes(uint32_t cols, uint32_t groups) {
+        return kDepth * (V > 1 ? NV * kThreads * kPackBytes : groups * LineBytes(cols));
+    }
+    __device__ __forceinline__ Ring(const void* base, uint64_t pitch, uint32_t rows, uint32_t cols_, char* memory, const Group& g, const Share& share) {
+        next = now = static_cast<const T*>(base) + share.first * pitch + (V > 1 ? g.lane * V : 0U);
+        step = share.stride * pitch;
+        cols = cols_;
+        line_bytes = LineBytes(cols_);
+        slots = memory + (V > 1 ? threadIdx.x * kPackBytes : g.index * line_bytes);
+        least = reinterpret_cast<uintptr_t>(base);
+        most = reinterpret_cast<uintptr_t>(static_cast<const T*>(base) + (rows - 1ULL) * pitch + cols_);
+    }
+    __device__ __forceinline__ char* Slot(const Group& g, uint32_t turn, int i) const {
+        if constexpr (V > 1) return slots + (turn * NV + i) * (kThreads * kPackBytes);
+        else return slots + turn * g.count * line_bytes;
+    }
+    __device__ __forceinline__ void Fetch(const Group& g, uint32_t turn, bool in) {
+        if (in) {
+            if constexpr (V > 1) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (PackColumn<V>(g, i) < cols) CopyAsync<kPackBytes>(static_cast<uint32_t>(__cvta_generic_to_shared(Slot(g, turn, i))), next + i * g.lanes * V);
+            } else {
+                const uintptr_t begin = reinterpret_cast<uintptr_t>(next), end = begin + static_cast<uintptr_t>(cols) * sizeof(T);
+                char* to = Slot(g, turn, 0) + 16U * g.lane;
+                for (uintptr_t line = (begin & ~static_cast<uintptr_t>(15)) + 16U * g.lane; line < end; line += 16U * g.lanes, to += 16U * g.lanes) {
+                    if (line >= least && line + 16U <= most) {
+                        CopyAsync<16>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), reinterpret_cast<const void*>(line));
+                    } else {
+                        for (uintptr_t e = line < begin ? begin : line; e < end && e < line + 16U; e += sizeof(T))
+                            *reinterpret_cast<T*>(to + (e - line)) = *reinterpret_cast<const T*>(e);
+                    }
+                }
+            }
+        }
+        next += step;
+    }
+    // This thread's elements of a row that has arrived; zeros beyond the row's end, and where there is no row.
+    __device__ __forceinline__ void Read(Held<NV * V>& out, const Group& g, uint32_t turn, bool in) {
+        const char* line = V > 1 ? nullptr : Slot(g, turn, 0) + (reinterpret_cast<uintptr_t>(now) & 15U);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t c = PackColumn<V>(g, i);
+            const T* from = V > 1 ? reinterpret_cast<const T*>(Slot(g, turn, i)) : reinterpret_cast<const T*>(line) + c;
+            Pack<T, V> p;
+            using W = typename Word<kPackBytes>::type;
+            *reinterpret_cast<W*>(&p) = W{};
+            if (in && c < cols) p = LoadPack<T, V>(from);
+#pragma unroll
+            for (int j = 0; j < V; ++j) out.Set(i * V + j, ToFloat(p.v[j]));
+        }
+        now += step;
+    }
+};
+template <class T, int V, int E>
+__device__ __forceinline__ Pack<T, V> PackOf(const Held<E>& v, int i) {
+    Pack<T, V> p;
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.v[j] = FromFloat<T>(v.Get(i * V + j));
+    return p;
+}
+// `value` where the thread's elements are in the row, zero where they are not.
+template <int V, int NV>
+__device__ __forceinline__ void InRow(Held<NV * V>& out, const Group& g, uint32_t cols, float value) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const float v = PackColumn<V>(g, i) < cols ? value : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) out.Set(i * V + j, v);
+    }
+}
+// A vector of columns that may begin anywhere; `none` for no vector, zero beyond the row's end.
+template <int V, int NV>
+__device__ __forceinline__ void LoadColumns(Held<NV * V>& out, const Group& g, uint32_t cols, const float* p, float none) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t c = PackColumn<V>(g, i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) out.Set(i * V + j, c < cols ? (p != nullptr ? p[c + j] : none) : 0.0f);
+    }
+}
+template <int E>
+__device__ __forceinline__ float SumOf(const Held<E>& v) {
+    float2 s = v.pair[0];
+#pragma unroll
+    for (int k = 1; k < Held<E>::kPairs; ++k) s = Add2(s, v.pair[k]);
+    return s.x + s.y;
+}
+// Everybody of the group sees what the group copied, or has read what it will overwrite.
+__device__ __forceinline__ void GroupBarrier(const Group& g) {
+    if (g.lanes <= 32U) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1U + g.index), "r"(g.lanes) : "memory");
+}
 
 // ---- host side: how a row is cut
-constexpr uint32_t kMostLanes = 512;
+constexpr uint32_t kMostLanes = 512, kElements = 16;
 struct Cut {
-    int v, nv;           // elements of a pack, packs a thread
+    int nv;              // packs a thread: 1, 2, 4, 8 or 16
     uint32_t lanes, threads;
-    bool stream;         // wider than the registers of a CTA hold
+    bool stream;         // wider than a CTA holds
 };
 inline uint32_t PowerOfTwo(uint32_t n) {
     uint32_t p = 1;
     while (p < n) p <<= 1;
     return p;
 }
-// elements: what a thread can hold. Packs a thread are 1, 2, 4, 8 or 16.
-inline Cut CutRow(uint32_t cols, int v, int elements) {
-    const uint32_t packs = (cols - 1U) / static_cast<uint32_t>(v) + 1U, most = static_cast<uint32_t>(elements / v);
-    Cut c{v, 1, 1, 256, false};
-    if (packs <= 32U) {
-        c.lanes = PowerOfTwo(packs);
-    } else if (packs <= 32U * most) {
-        c.lanes = 32;
-        c.nv = static_cast<int>(PowerOfTwo((packs + 31U) / 32U));
-    } else {
-        c.nv = static_cast<int>(most);
-        if (packs > most * kMostLanes) {
-            c.stream = true;
-            return c;
-        }
-        c.lanes = PowerOfTwo((packs - 1U) / most + 1U);
-        if (c.lanes > c.threads) c.threads = c.lanes;
+// As few lanes a row as can hold it, which makes the reductions short, or more where the rows are too few to fill the chip's threads.
+inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v) {
+    const uint32_t packs = (cols - 1U) / v + 1U, most = kElements / v;
+    Cut c{1, 1, 256, false};
+    if (packs > most * kMostLanes) {
+        c.stream = true;
+        return c;
     }
+    c.lanes = PowerOfTwo((packs - 1U) / most + 1U);
+    if (v == 1U && c.lanes < 4U) c.lanes = 4;  // (a line of 16 bytes and more a row: not too many rows a CTA)
+    while (c.lanes < 256U && c.lanes < packs && static_cast<uint64_t>(rows) * c.lanes < 148ULL * 512ULL) c.lanes <<= 1;
+    c.nv = static_cast<int>(PowerOfTwo((packs - 1U) / c.lanes + 1U));
+    if (c.lanes > c.threads) c.threads = c.lanes;
     return c;
+}
+// Dynamic shared memory beyond 48 KB is an attribute of a kernel on a device: set on the first launch there.
+template <class Kernel>
+inline bool AllowShared(Kernel kernel, std::atomic<uint64_t>& done, int bytes) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return false;
+    const uint64_t bit = 1ULL << device;
+    if ((done.load(std::memory_order_relaxed) & bit) != 0) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 inline uint32_t TypeBytes(int32_t type) { return type == MGT_F32 ? 4U : 2U; }
 inline bool RowsAligned(const void* p, uint64_t pitch, uint32_t rows, int32_t type, int v) {
-    const uint64_t bytes = TypeBytes(type) * static_cast<uint64_t>(v), unit = bytes > 16U ? 16U : bytes;
-    return (reinterpret_cast<uintptr_t>(p) % unit) == 0 && (rows <= 1U || (pitch * TypeBytes(type)) % unit == 0);
+    const uint64_t bytes = TypeBytes(type) * static_cast<uint64_t>(v);
+    return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (rows <= 1U || (pitch * TypeBytes(type)) % bytes == 0);
 }
 
 }  // namespace ln

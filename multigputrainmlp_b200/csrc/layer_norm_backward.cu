@@ -10,81 +10,92 @@ namespace {
 
 constexpr uint32_t kSums = 3;
 constexpr uint32_t kMostCtas = 296;     // partial rows at most: two CTAs on each of 148 SMs
+constexpr int kMostShared = 200 << 10;
 constexpr uint32_t kColumnSlices = 37;  // widest rows: slices of the batch that the column sums are taken over
 
+template <class Tdy, class Tx, int V, int NV>
+constexpr int kDepth = V == 1 ? 2 : NV * V * (sizeof(Tdy) + sizeof(Tx)) >= 64 ? 3 : 6;
+
 template <class Tdy, class Tx, class Tdx, int V, int NV, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
 BackwardKernel(const Backward a) {
-    extern __shared__ float lanes_sums[];  // [groups][cols], more than one group
+    extern __shared__ __align__(16) char memory[];  // the rings; at the end [groups][cols] sums, where there is more than one group
     __shared__ float2 buffer[2 * (kThreads / 32)];
+    constexpr int D = kDepth<Tdy, Tx, V, NV>, kPairs = Held<NV * V>::kPairs;
+    using RingDy = Ring<Tdy, V, NV, kThreads, D>;
     Group g = MakeGroup(a.lanes, buffer);
-    const uint32_t stride = gridDim.x * g.count;
-    const float cols = static_cast<float>(a.cols);
+    const Share share = MakeShare(g, a.rows);
+    RingDy ring_dy(a.dy, a.dy_pitch, a.rows, a.cols, memory, g, share);
+    Ring<Tx, V, NV, kThreads, D> ring_x(a.x, a.x_pitch, a.rows, a.cols, memory + RingDy::Bytes(a.cols, g.count), g, share);
+    const float per_col = 1.0f / static_cast<float>(a.cols);
+    Tdx* dx = static_cast<Tdx*>(a.dx) + share.first * a.dx_pitch + g.lane * V;
+    const uint64_t dx_step = share.stride * a.dx_pitch;
     dependent_begin();
-    float gamma[NV][V], sums[kSums][NV][V] = {};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t c = PackColumn<V>(g, i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) gamma[i][j] = c + j < a.cols ? (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) : 0.0f;
+    for (int d = 0; d < D; ++d) {
+        ring_dy.Fetch(g, d, d < share.mine);
+        ring_x.Fetch(g, d, d < share.mine);
+        CopiesEnd();
     }
-    const Tdy* dy = static_cast<const Tdy*>(a.dy);
-    const Tx* x = static_cast<const Tx*>(a.x);
-    Tdx* dx = static_cast<Tdx*>(a.dx);
-    Pack<Tdy, V> next_dy[NV];
-    Pack<Tx, V> next_x[NV];
     float next_mean = 0.0f, next_rstd = 0.0f;
-    auto load = [&](uint64_t row) {
-        const bool in = row < a.rows;
-        if (in) {
+    if (share.mine != 0U) {
+        next_mean = a.mean[share.first];
+        next_rstd = a.rstd[share.first];
+    }
+    Held<NV * V> gamma, sums[kSums], gy, xhat;
+    LoadColumns<V, NV>(gamma, g, a.cols, a.gamma, 1.0f);
+#pragma unroll
+    for (uint32_t n = 0; n < kSums; ++n)
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) sums[n].pair[k] = Both(0.0f);
+    uint32_t slot = 0, row = share.first;
+    for (uint32_t t = 0; t < share.turns; ++t) {
+        const bool in = t < share.mine;
+        const float mean = in ? next_mean : 0.0f, rstd = in ? next_rstd : 0.0f;  // (a row that is not there adds nothing to the sums)
+        row += share.stride;
+        if (t + 1U < share.mine) {
             next_mean = a.mean[row];
             next_rstd = a.rstd[row];
         }
+        CopiesWait<D - 1>();
+        if (V == 1) GroupBarrier(g);
+        ring_dy.Read(gy, g, slot, in);
+        ring_x.Read(xhat, g, slot, in);
+        Held<NV * V> less;
+        InRow<V, NV>(less, g, a.cols, -mean);
+        float2 s1 = Both(0.0f), s2 = Both(0.0f);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i), valid = in ? PackValid(c, a.cols) : 0U;
-            LoadPack<Tdy, V>(next_dy[i], dy + row * a.dy_pitch + c, valid);
-            LoadPack<Tx, V>(next_x[i], x + row * a.x_pitch + c, valid);
+        for (int k = 0; k < kPairs; ++k) {
+            xhat.pair[k] = Mul2(Add2(xhat.pair[k], less.pair[k]), Both(rstd));
+            sums[0].pair[k] = Fma2(gy.pair[k], xhat.pair[k], sums[0].pair[k]);
+            sums[1].pair[k] = Add2(gy.pair[k], sums[1].pair[k]);
+            gy.pair[k] = Mul2(gy.pair[k], gamma.pair[k]);
+            s1 = Add2(s1, gy.pair[k]);
+            s2 = Fma2(gy.pair[k], xhat.pair[k], s2);
         }
-    };
-    uint64_t row = static_cast<uint64_t>(blockIdx.x) * g.count + g.index;
-    const uint64_t warp_first = g.lanes < 32U ? row - (g.index & (32U / g.lanes - 1U)) : row;  // the loop's bound is a warp's
-    const uint64_t ahead = row - warp_first;
-    load(row);
-    for (uint64_t first = warp_first; first < a.rows; first += stride) {
-        row = first + ahead;
-        const float mean = next_mean, rstd = next_rstd;
-        float xhat[NV][V], d[NV][V], s1 = 0.0f, s2 = 0.0f;
+        float s[2] = {s1.x + s1.y, s2.x + s2.y};
+        Reduce(g, s);
+        if (V == 1) GroupBarrier(g);  // (everybody has what it read of the slot: the sums needed it)
+        ring_dy.Fetch(g, slot, t + D < share.mine);
+        ring_x.Fetch(g, slot, t + D < share.mine);
+        CopiesEnd();
+        slot = slot + 1U == D ? 0U : slot + 1U;
+        if (in) {
+            const float2 c1 = Both(-s[0] * per_col), c2 = Both(-s[1] * per_col), scale = Both(rstd);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                d[i][j] = ToFloat(next_dy[i].v[j]);
-                xhat[i][j] = c + j < a.cols ? (ToFloat(next_x[i].v[j]) - mean) * rstd : 0.0f;
-                const float t = d[i][j] * gamma[i][j];
-                s1 += t;
-                s2 += t * xhat[i][j];
+            for (int k = 0; k < kPairs; ++k) {
+                gy.pair[k] = Mul2(scale, Fma2(xhat.pair[k], c2, Add2(gy.pair[k], c1)));  // (rstd last: it is large where the differences are small)
+                sums[2].pair[k] = Add2(gy.pair[k], sums[2].pair[k]);  // (before it is rounded to dx's type; beyond the row's end nobody looks)
             }
-        }
-        load(row + stride);  // the next row is on its way while this one is reduced
-        const float2 total = Reduce(g, s1, s2);
-        if (row >= a.rows) continue;
-        const float c1 = total.x / cols, c2 = total.y / cols;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i), valid = PackValid(c, a.cols);
-            float out[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                out[j] = rstd * (d[i][j] * gamma[i][j] - c1 - xhat[i][j] * c2);
-                sums[0][i][j] += d[i][j] * xhat[i][j];
-                sums[1][i][j] += d[i][j];
-                sums[2][i][j] += out[j];  // (before it is rounded to dx's type)
-            }
-            StorePack<Tdx, V>(dx + row * a.dx_pitch + c, out, valid);
+            for (int i = 0; i < NV; ++i)
+                if (PackColumn<V>(g, i) < a.cols) StorePack<Tdx, V>(dx + i * g.lanes * V, PackOf<Tdx, V>(gy, i));
         }
+        dx += dx_step;
     }
+    CopiesWait<0>();
+    float* lanes_sums = reinterpret_cast<float*>(memory);
+    __syncthreads();  // (the rings are no longer read)
     // this CTA's column sums: the groups in order
     float* partial = a.partial + static_cast<uint64_t>(blockIdx.x) * kSums * a.cols;
 #pragma unroll
@@ -97,7 +108,7 @@ BackwardKernel(const Backward a) {
             const uint32_t c = PackColumn<V>(g, i);
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (c + j < a.cols) mine[c + j] = sums[k][i][j];
+                if (c < a.cols) mine[c + j] = sums[k].Get(i * V + j);
         }
         if (g.count > 1U) {
             __syncthreads();
@@ -149,22 +160,20 @@ StreamMeansKernel(const Backward a, float2* means) {
         const Tdy* dy = static_cast<const Tdy*>(a.dy) + row * a.dy_pitch;
         const Tx* x = static_cast<const Tx*>(a.x) + row * a.x_pitch;
         const float mean = a.mean[row], rstd = a.rstd[row];
-        float s1 = 0.0f, s2 = 0.0f;
+        float s[2] = {0.0f, 0.0f};
 #pragma unroll 2
         for (uint32_t c = threadIdx.x * V; c < a.cols; c += step) {
-            Pack<Tdy, V> pd;
-            Pack<Tx, V> px;
-            LoadPack<Tdy, V>(pd, dy + c, a.cols - c);
-            LoadPack<Tx, V>(px, x + c, a.cols - c);
+            const Pack<Tdy, V> pd = LoadPack<Tdy, V>(dy + c);
+            const Pack<Tx, V> px = LoadPack<Tx, V>(x + c);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float t = c + j < a.cols ? ToFloat(pd.v[j]) * (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) : 0.0f;
-                s1 += t;
-                s2 += t * ((ToFloat(px.v[j]) - mean) * rstd);
+                const float t = ToFloat(pd.v[j]) * (a.gamma != nullptr ? a.gamma[c + j] : 1.0f);
+                s[0] += t;
+                s[1] += t * ((ToFloat(px.v[j]) - mean) * rstd);
             }
         }
-        const float2 total = Reduce(g, s1, s2);
-        if (threadIdx.x == 0U) means[row] = make_float2(total.x / cols, total.y / cols);
+        Reduce(g, s);
+        if (threadIdx.x == 0U) means[row] = make_float2(s[0] / cols, s[1] / cols);
     }
 }
 // ... then, a tile of columns and a slice of the rows at a time, dx and the column sums.
@@ -174,36 +183,32 @@ StreamColumnsKernel(const Backward a, const float2* means, uint32_t rows_each) {
     const uint32_t c = (blockIdx.x * 256U + threadIdx.x) * V;
     dependent_begin();
     if (c >= a.cols) return;
-    const uint32_t valid = a.cols - c;
     const uint64_t r0 = static_cast<uint64_t>(blockIdx.y) * rows_each, r1 = min(static_cast<uint64_t>(a.rows), r0 + rows_each);
     float gamma[V], sums[kSums][V] = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j) gamma[j] = j < valid ? (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) : 0.0f;
+    for (int j = 0; j < V; ++j) gamma[j] = a.gamma != nullptr ? a.gamma[c + j] : 1.0f;
 #pragma unroll 4
     for (uint64_t row = r0; row < r1; ++row) {
-        Pack<Tdy, V> pd;
-        Pack<Tx, V> px;
-        LoadPack<Tdy, V>(pd, static_cast<const Tdy*>(a.dy) + row * a.dy_pitch + c, valid);
-        LoadPack<Tx, V>(px, static_cast<const Tx*>(a.x) + row * a.x_pitch + c, valid);
+        const Pack<Tdy, V> pd = LoadPack<Tdy, V>(static_cast<const Tdy*>(a.dy) + row * a.dy_pitch + c);
+        const Pack<Tx, V> px = LoadPack<Tx, V>(static_cast<const Tx*>(a.x) + row * a.x_pitch + c);
         const float mean = a.mean[row], rstd = a.rstd[row];
         const float2 m = means[row];
-        float out[V];
+        Pack<Tdx, V> out;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float d = ToFloat(pd.v[j]), xhat = (ToFloat(px.v[j]) - mean) * rstd;
-            out[j] = rstd * (d * gamma[j] - m.x - xhat * m.y);
+            const float d = ToFloat(pd.v[j]), xhat = (ToFloat(px.v[j]) - mean) * rstd, o = rstd * (d * gamma[j] - m.x - xhat * m.y);
             sums[0][j] += d * xhat;
             sums[1][j] += d;
-            sums[2][j] += out[j];
+            sums[2][j] += o;
+            out.v[j] = FromFloat<Tdx>(o);
         }
-        StorePack<Tdx, V>(static_cast<Tdx*>(a.dx) + row * a.dx_pitch + c, out, valid);
+        StorePack<Tdx, V>(static_cast<Tdx*>(a.dx) + row * a.dx_pitch + c, out);
     }
     float* partial = a.partial + static_cast<uint64_t>(blockIdx.y) * kSums * a.cols;
 #pragma unroll
     for (uint32_t k = 0; k < kSums; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < valid) partial[k * a.cols + c + j] = sums[k][j];
+        for (int j = 0; j < V; ++j) partial[k * a.cols + c + j] = sums[k][j];
 }
 
 void SumPartialRows(const Backward& a, uint32_t rows, LaunchOn on, uint32_t* launches) {
@@ -211,25 +216,26 @@ void SumPartialRows(const Backward& a, uint32_t rows, LaunchOn on, uint32_t* lau
     ++*launches;
 }
 
-// Elements that a thread holds of a row: with an fp32 operand 8, else 16. Beside them are the next row's, gamma and three sums a column.
-template <class Tdy, class Tx>
-constexpr int kElements = sizeof(Tdy) == 4 || sizeof(Tx) == 4 ? 8 : 16;
-
 template <class Tdy, class Tx, class Tdx, int V, int NV, int kThreads>
-void Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
+mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint32_t groups = cut.threads / cut.lanes;
     const uint64_t want = (static_cast<uint64_t>(a.rows) + groups - 1U) / groups;
-    const uint32_t ctas = static_cast<uint32_t>(want < kMostCtas ? want : kMostCtas);
+    const uint32_t most = cut.threads == 256U ? kMostCtas : kMostCtas / 2U;
+    const uint32_t ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
-    const size_t smem = groups > 1U ? static_cast<size_t>(groups) * a.cols * sizeof(float) : 0;
+    constexpr int D = kDepth<Tdy, Tx, V, NV>;
+    const uint32_t rings = Ring<Tdy, V, NV, kThreads, D>::Bytes(a.cols, groups) + Ring<Tx, V, NV, kThreads, D>::Bytes(a.cols, groups);
+    const uint32_t sums = groups > 1U ? groups * a.cols * 4U : 0U, smem = rings > sums ? rings : sums;
+    static std::atomic<uint64_t> allowed{0};
+    if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, V, NV, kThreads>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
     Launch(BackwardKernel<Tdy, Tx, Tdx, V, NV, kThreads>, ctas, cut.threads, smem, on, a);
     ++*launches;
     if (ctas > 1U && (a.sums[0] != nullptr || a.sums[1] != nullptr || a.sums[2] != nullptr)) SumPartialRows(a, ctas, on, launches);
+    return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
 }
 template <class Tdy, class Tx, class Tdx, int V>
-void RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
-    constexpr int kE = kElements<Tdy, Tx>;
-    const Cut cut = CutRow(a.cols, V, kE);
+mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
+    const Cut cut = CutRow(a.rows, a.cols, V);
     if (cut.stream) {
         float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kMostCtas) * kSums * a.cols);
         Launch(StreamMeansKernel<Tdy, Tx, V>, a.rows < 296U ? a.rows : 296U, 1024, 0, on, a, means);
@@ -238,43 +244,46 @@ void RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
         Launch(StreamColumnsKernel<Tdy, Tx, Tdx, V>, dim3((a.cols - 1U) / (256U * V) + 1U, used), 256, 0, LaunchOn(on.stream, true), a, static_cast<const float2*>(means), rows_each);
         *launches += 2;
         SumPartialRows(a, used, on, launches);
-        return;
+        return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
-    constexpr int kMost = kE / V, kFew = V == 1 ? 4 : 2;
-    if (cut.threads > 256U) Run<Tdy, Tx, Tdx, V, kMost, 512>(a, cut, on, launches);
-    else if (cut.nv == 1) Run<Tdy, Tx, Tdx, V, 1, 256>(a, cut, on, launches);
-    else if (cut.nv <= kFew) Run<Tdy, Tx, Tdx, V, kFew, 256>(a, cut, on, launches);
-    else Run<Tdy, Tx, Tdx, V, kMost, 256>(a, cut, on, launches);
+    constexpr int kMost = kElements / V, kFew = V == 1 ? 4 : 2;  // packs a thread that there are kernels for, besides one
+    if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, V, kMost, 512>(a, cut, on, launches);
+    if (cut.nv == 1) return Run<Tdy, Tx, Tdx, V, 1, 256>(a, cut, on, launches);
+    if (cut.nv <= kFew) return Run<Tdy, Tx, Tdx, V, kFew, 256>(a, cut, on, launches);
+    return Run<Tdy, Tx, Tdx, V, kMost, 256>(a, cut, on, launches);
 }
 template <class Tdy, class Tx, class Tdx>
-void RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {
-    constexpr int kV = sizeof(Tdy) == 2 && sizeof(Tx) == 2 && sizeof(Tdx) == 2 ? 8 : 4;
-    if (RowsAligned(a.dy, a.dy_pitch, a.rows, dy_type, kV) && RowsAligned(a.x, a.x_pitch, a.rows, x_type, kV) && RowsAligned(a.dx, a.dx_pitch, a.rows, dx_type, kV))
-        RunByWidth<Tdy, Tx, Tdx, kV>(a, on, launches);
-    else RunByWidth<Tdy, Tx, Tdx, 1>(a, on, launches);
+mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {
+    auto whole = [&](int v) {
+        return a.cols % v == 0 && RowsAligned(a.dy, a.dy_pitch, a.rows, dy_type, v) && RowsAligned(a.x, a.x_pitch, a.rows, x_type, v) &&
+               RowsAligned(a.dx, a.dx_pitch, a.rows, dx_type, v);
+    };
+    if constexpr (sizeof(Tdy) == 2 && sizeof(Tx) == 2 && sizeof(Tdx) == 2)
+        if (whole(8)) return RunByWidth<Tdy, Tx, Tdx, 8>(a, on, launches);
+    if (whole(4)) return RunByWidth<Tdy, Tx, Tdx, 4>(a, on, launches);
+    return RunByWidth<Tdy, Tx, Tdx, 1>(a, on, launches);
 }
 
 }  // namespace
 
 uint64_t BackwardFloats(uint32_t rows, uint32_t cols) {
-    return static_cast<uint64_t>(kMostCtas) * kSums * cols + (cols > 8U * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
+    return static_cast<uint64_t>(kMostCtas) * kSums * cols + (cols > kElements * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
 }
 
 mgt_status_t LaunchBackward(Backward a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {
     auto is = [&](int32_t dy, int32_t x, int32_t dx) { return dy_type == dy && x_type == x && dx_type == dx; };
     using H = __half;
     using B = __nv_bfloat16;
-    if (is(MGT_F32, MGT_F32, MGT_F32)) RunTyped<float, float, float>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_F32, MGT_F32, MGT_F16)) RunTyped<float, float, H>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_F32, MGT_F32, MGT_BF16)) RunTyped<float, float, B>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_F16, MGT_F32, MGT_F32)) RunTyped<H, float, float>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_BF16, MGT_F32, MGT_F32)) RunTyped<B, float, float>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_F16, MGT_F16, MGT_F16)) RunTyped<H, H, H>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_F32, MGT_F16, MGT_F16)) RunTyped<float, H, H>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_BF16, MGT_BF16, MGT_BF16)) RunTyped<B, B, B>(a, dy_type, x_type, dx_type, on, launches);
-    else if (is(MGT_F32, MGT_BF16, MGT_BF16)) RunTyped<float, B, B>(a, dy_type, x_type, dx_type, on, launches);
-    else return MGT_INVALID_CONFIG;
-    return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
+    if (is(MGT_F32, MGT_F32, MGT_F32)) return RunTyped<float, float, float>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_F32, MGT_F32, MGT_F16)) return RunTyped<float, float, H>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_F32, MGT_F32, MGT_BF16)) return RunTyped<float, float, B>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_F16, MGT_F32, MGT_F32)) return RunTyped<H, float, float>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_BF16, MGT_F32, MGT_F32)) return RunTyped<B, float, float>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_F16, MGT_F16, MGT_F16)) return RunTyped<H, H, H>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_F32, MGT_F16, MGT_F16)) return RunTyped<float, H, H>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_BF16, MGT_BF16, MGT_BF16)) return RunTyped<B, B, B>(a, dy_type, x_type, dx_type, on, launches);
+    if (is(MGT_F32, MGT_BF16, MGT_BF16)) return RunTyped<float, B, B>(a, dy_type, x_type, dx_type, on, launches);
+    return MGT_INVALID_CONFIG;
 }
 
 }  // namespace ln

@@ -10,92 +10,89 @@ namespace {
 struct Moments {
     float mean, shift, rstd;
 };
-__device__ __forceinline__ Moments Finish(float first, float2 sums, float cols, float eps) {
-    const float shift = sums.x / cols;
-    const float var = sums.y / cols - shift * shift;
-    return {first + shift, shift, 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps)};  // (a NaN stays one)
+__device__ __forceinline__ Moments Finish(float first, const float (&sums)[2], float per_col, float eps) {
+    const float shift = sums[0] * per_col;
+    const float var = sums[1] * per_col - shift * shift, v = (var < 0.0f ? 0.0f : var) + eps;  // (a NaN stays one)
+    const float r = rsqrtf(v);
+    return {first + shift, shift, r * fmaf(-0.5f * v * r, r, 1.5f)};  // one Newton step: to an ulp, at a tenth of a root's and a division's price
 }
+
+template <class Tx, int V, int NV>
+constexpr int kDepth = V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : NV * V * sizeof(Tx) >= 64 ? 3 : NV * V * sizeof(Tx) >= 32 ? 5 : 8;
+constexpr uint32_t kCtasPerSm = 3;
 
 // kTower: x is a layer's output before its normalisation, the normalised row is added to the fp32 residual stream, and what a ReLU leaves
 // goes to the stream and, as the next product's operand, to y.
 template <class Tx, class Ty, int V, int NV, int kThreads, bool kTower>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? kCtasPerSm : 1)
 ForwardKernel(const Forward a) {
+    extern __shared__ __align__(16) char memory[];
     __shared__ float2 buffer[2 * (kThreads / 32)];
+    constexpr int D = kDepth<Tx, V, NV>, kPairs = Held<NV * V>::kPairs;
     Group g = MakeGroup(a.lanes, buffer);
-    const uint32_t stride = gridDim.x * g.count;
-    const float cols = static_cast<float>(a.cols);
+    const Share share = MakeShare(g, a.rows);
+    Ring<Tx, V, NV, kThreads, D> ring(a.x, a.x_pitch, a.rows, a.cols, memory, g, share);
+    const float per_col = 1.0f / static_cast<float>(a.cols);
+    Ty* y = static_cast<Ty*>(a.y) + share.first * a.y_pitch + g.lane * V;
+    float* state = kTower ? a.state + share.first * a.x_pitch + g.lane * V : nullptr;
+    const uint64_t y_step = share.stride * a.y_pitch, state_step = share.stride * a.x_pitch;
     dependent_begin();
-    float gamma[NV][V], beta[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t c = PackColumn<V>(g, i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            gamma[i][j] = c + j < a.cols ? (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) : 0.0f;
-            beta[i][j] = c + j < a.cols && a.beta != nullptr ? a.beta[c + j] : 0.0f;
-        }
+    for (int d = 0; d < D; ++d) {
+        ring.Fetch(g, d, d < share.mine);
+        CopiesEnd();
     }
-    const Tx* x = static_cast<const Tx*>(a.x);
-    Ty* y = static_cast<Ty*>(a.y);
-    Pack<Tx, V> next[NV];
-    auto load = [&](uint64_t row) {
+    Held<NV * V> gamma, beta, m, v;
+    LoadColumns<V, NV>(gamma, g, a.cols, a.gamma, 1.0f);
+    LoadColumns<V, NV>(beta, g, a.cols, a.beta, 0.0f);
+    uint32_t slot = 0, row = share.first;
+    for (uint32_t t = 0; t < share.turns; ++t) {
+        const bool in = t < share.mine;
+        CopiesWait<D - 1>();
+        if (V == 1) GroupBarrier(g);
+        ring.Read(v, g, slot, in);
+        float sum[1] = {SumOf(v)};
+        Reduce(g, sum);
+        if (V == 1) GroupBarrier(g);  // (everybody has what it read of the slot: the sum needed it)
+        ring.Fetch(g, slot, t + D < share.mine);
+        CopiesEnd();
+        slot = slot + 1U == D ? 0U : slot + 1U;
+        const float first = sum[0] * per_col;
+        InRow<V, NV>(m, g, a.cols, -first);
+        float2 s1 = Both(0.0f), s2 = Both(0.0f);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i);
-            LoadPack<Tx, V>(next[i], x + row * a.x_pitch + c, row < a.rows ? PackValid(c, a.cols) : 0U);
+        for (int k = 0; k < kPairs; ++k) {
+            v.pair[k] = Add2(v.pair[k], m.pair[k]);
+            s1 = Add2(s1, v.pair[k]);
+            s2 = Fma2(v.pair[k], v.pair[k], s2);
         }
-    };
-    uint64_t row = static_cast<uint64_t>(blockIdx.x) * g.count + g.index;
-    const uint64_t warp_first = g.lanes < 32U ? row - (g.index & (32U / g.lanes - 1U)) : row;  // the loop's bound is a warp's
-    const uint64_t ahead = row - warp_first;
-    load(row);
-    for (uint64_t first = warp_first; first < a.rows; first += stride) {
-        row = first + ahead;
-        float v[NV][V];
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v[i][j] = ToFloat(next[i].v[j]);  // (zero beyond the row's end)
-                sum += v[i][j];
+        float s[2] = {s1.x + s1.y, s2.x + s2.y};
+        Reduce(g, s);
+        const Moments mo = Finish(first, s, per_col, a.eps);
+        if (in) {
+            if (g.lane == 0U) {
+                if (a.mean != nullptr) a.mean[row] = mo.mean;
+                if (a.rstd != nullptr) a.rstd[row] = mo.rstd;
             }
-        load(row + stride);  // the next row is on its way while this one is reduced
-        const float m = Reduce(g, sum, 0.0f).x / cols;
-        float s1 = 0.0f, s2 = 0.0f;
+            const float2 rstd = Both(mo.rstd), off = Both(-mo.shift * mo.rstd);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i);
+            for (int k = 0; k < kPairs; ++k) v.pair[k] = Fma2(Fma2(v.pair[k], rstd, off), gamma.pair[k], beta.pair[k]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v[i][j] = c + j < a.cols ? v[i][j] - m : 0.0f;
-                s1 += v[i][j];
-                s2 += v[i][j] * v[i][j];
+            for (int i = 0; i < NV; ++i) {
+                if (PackColumn<V>(g, i) >= a.cols) continue;
+                const uint32_t at = i * g.lanes * V;
+                if (kTower) {
+                    const Pack<float, V> old = a.add ? LoadPack<float, V>(state + at) : Pack<float, V>{};
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v.Set(i * V + j, fmaxf(old.v[j] + v.Get(i * V + j), 0.0f));
+                    StorePack<float, V>(state + at, PackOf<float, V>(v, i));
+                }
+                StorePack<Ty, V>(y + at, PackOf<Ty, V>(v, i));
             }
         }
-        const Moments mo = Finish(m, Reduce(g, s1, s2), cols, a.eps);
-        if (row >= a.rows) continue;
-        if (g.lane == 0U) {
-            if (a.mean != nullptr) a.mean[row] = mo.mean;
-            if (a.rstd != nullptr) a.rstd[row] = mo.rstd;
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i), valid = PackValid(c, a.cols);
-            float out[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) out[j] = (v[i][j] - mo.shift) * mo.rstd * gamma[i][j] + beta[i][j];
-            if (kTower) {
-                float* state = a.state + row * a.x_pitch + c;
-                Pack<float, V> old;
-                LoadPack<float, V>(old, state, a.add ? valid : 0U);
-#pragma unroll
-                for (int j = 0; j < V; ++j) out[j] = fmaxf(old.v[j] + out[j], 0.0f);
-                StorePack<float, V>(state, out, valid);
-            }
-            StorePack<Ty, V>(y + row * a.y_pitch + c, out, valid);
-        }
+        y += y_step;
+        if (kTower) state += state_step;
+        row += share.stride;
     }
 }
 
@@ -105,107 +102,111 @@ __global__ void __launch_bounds__(1024)
 StreamForwardKernel(const Forward a) {
     __shared__ float2 buffer[2 * 32];
     Group g = MakeGroup(blockDim.x, buffer);
-    const float cols = static_cast<float>(a.cols);
+    const float per_col = 1.0f / static_cast<float>(a.cols);
     const uint32_t step = blockDim.x * V;
     dependent_begin();
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const Tx* x = static_cast<const Tx*>(a.x) + row * a.x_pitch;
         Ty* y = static_cast<Ty*>(a.y) + row * a.y_pitch;
-        float sum = 0.0f;
+        float sum[1] = {0.0f};
 #pragma unroll 4
         for (uint32_t c = threadIdx.x * V; c < a.cols; c += step) {
-            Pack<Tx, V> p;
-            LoadPack<Tx, V>(p, x + c, a.cols - c);
+            const Pack<Tx, V> p = LoadPack<Tx, V>(x + c);
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum += ToFloat(p.v[j]);
+            for (int j = 0; j < V; ++j) sum[0] += ToFloat(p.v[j]);
         }
-        const float m = Reduce(g, sum, 0.0f).x / cols;
-        float s1 = 0.0f, s2 = 0.0f;
+        Reduce(g, sum);
+        const float m = sum[0] * per_col;
+        float s[2] = {0.0f, 0.0f};
 #pragma unroll 4
         for (uint32_t c = threadIdx.x * V; c < a.cols; c += step) {
-            Pack<Tx, V> p;
-            LoadPack<Tx, V>(p, x + c, a.cols - c);
+            const Pack<Tx, V> p = LoadPack<Tx, V>(x + c);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = c + j < a.cols ? ToFloat(p.v[j]) - m : 0.0f;
-                s1 += d;
-                s2 += d * d;
+                const float d = ToFloat(p.v[j]) - m;
+                s[0] += d;
+                s[1] += d * d;
             }
         }
-        const Moments mo = Finish(m, Reduce(g, s1, s2), cols, a.eps);
+        Reduce(g, s);
+        const Moments mo = Finish(m, s, per_col, a.eps);
         if (threadIdx.x == 0U) {
             if (a.mean != nullptr) a.mean[row] = mo.mean;
             if (a.rstd != nullptr) a.rstd[row] = mo.rstd;
         }
 #pragma unroll 2
         for (uint32_t c = threadIdx.x * V; c < a.cols; c += step) {
-            Pack<Tx, V> p;
-            LoadPack<Tx, V>(p, x + c, a.cols - c);
-            float out[V];
+            const Pack<Tx, V> p = LoadPack<Tx, V>(x + c);
+            Pack<Ty, V> out;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const uint32_t k = min(c + j, a.cols - 1U);
-                out[j] = ((ToFloat(p.v[j]) - m) - mo.shift) * mo.rstd * (a.gamma != nullptr ? a.gamma[k] : 1.0f) + (a.beta != nullptr ? a.beta[k] : 0.0f);
-            }
-            StorePack<Ty, V>(y + c, out, a.cols - c);
+            for (int j = 0; j < V; ++j)
+                out.v[j] = FromFloat<Ty>(((ToFloat(p.v[j]) - m) - mo.shift) * mo.rstd * (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) + (a.beta != nullptr ? a.beta[c + j] : 0.0f));
+            StorePack<Ty, V>(y + c, out);
         }
     }
 }
 
-constexpr uint32_t kCtasPerSm = 3;
+constexpr int kMostShared = 110 << 10;
 
 template <class Tx, class Ty, int V, int NV, int kThreads, bool kTower>
-void Run(Forward a, const Cut& cut, LaunchOn on) {
+mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
     const uint32_t rows = cut.threads / cut.lanes;
     const uint64_t want = (static_cast<uint64_t>(a.rows) + rows - 1U) / rows;
     a.lanes = cut.lanes;
-    Launch(ForwardKernel<Tx, Ty, V, NV, kThreads, kTower>, static_cast<uint32_t>(want < 148U * kCtasPerSm ? want : 148U * kCtasPerSm), cut.threads, 0, on, a);
+    static std::atomic<uint64_t> allowed{0};
+    const uint32_t smem = Ring<Tx, V, NV, kThreads, kDepth<Tx, V, NV>>::Bytes(a.cols, rows);
+    if (!AllowShared(ForwardKernel<Tx, Ty, V, NV, kThreads, kTower>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
+    const uint32_t most = 148U * (cut.threads == 256U ? kCtasPerSm : 1U);
+    Launch(ForwardKernel<Tx, Ty, V, NV, kThreads, kTower>, static_cast<uint32_t>(want < most ? want : most), cut.threads, smem, on, a);
+    return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
 }
 template <class Tx, class Ty, int V>
-void RunByWidth(const Forward& a, LaunchOn on) {
-    const Cut cut = CutRow(a.cols, V, 16);
+mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
+    const Cut cut = CutRow(a.rows, a.cols, V);
     if (cut.stream) {
         Launch(StreamForwardKernel<Tx, Ty, V>, a.rows < 296U ? a.rows : 296U, 1024, 0, on, a);
-        return;
+        return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
-    constexpr int kMost = 16 / V, kFew = V == 1 ? 4 : 2;  // packs a thread that there are kernels for, besides one
-    if (cut.threads > 256U) Run<Tx, Ty, V, kMost, 512, false>(a, cut, on);
-    else if (cut.nv == 1) Run<Tx, Ty, V, 1, 256, false>(a, cut, on);
-    else if (cut.nv <= kFew) Run<Tx, Ty, V, kFew, 256, false>(a, cut, on);
-    else Run<Tx, Ty, V, kMost, 256, false>(a, cut, on);
+    constexpr int kMost = kElements / V, kFew = V == 1 ? 4 : 2;  // packs a thread that there are kernels for, besides one
+    if (cut.threads > 256U) return Run<Tx, Ty, V, kMost, 512, false>(a, cut, on);
+    if (cut.nv == 1) return Run<Tx, Ty, V, 1, 256, false>(a, cut, on);
+    if (cut.nv <= kFew) return Run<Tx, Ty, V, kFew, 256, false>(a, cut, on);
+    return Run<Tx, Ty, V, kMost, 256, false>(a, cut, on);
 }
 template <class Tx, class Ty>
-void RunTyped(const Forward& a, int32_t x_type, int32_t y_type, LaunchOn on) {
-    constexpr int kV = sizeof(Tx) == 2 && sizeof(Ty) == 2 ? 8 : 4;
-    if (RowsAligned(a.x, a.x_pitch, a.rows, x_type, kV) && RowsAligned(a.y, a.y_pitch, a.rows, y_type, kV)) RunByWidth<Tx, Ty, kV>(a, on);
-    else RunByWidth<Tx, Ty, 1>(a, on);
+mgt_status_t RunTyped(const Forward& a, int32_t x_type, int32_t y_type, LaunchOn on) {
+    auto whole = [&](int v) { return a.cols % v == 0 && RowsAligned(a.x, a.x_pitch, a.rows, x_type, v) && RowsAligned(a.y, a.y_pitch, a.rows, y_type, v); };
+    if constexpr (sizeof(Tx) == 2 && sizeof(Ty) == 2)
+        if (whole(8)) return RunByWidth<Tx, Ty, 8>(a, on);
+    if (whole(4)) return RunByWidth<Tx, Ty, 4>(a, on);
+    return RunByWidth<Tx, Ty, 1>(a, on);
 }
 
 }  // namespace
 
 mgt_status_t LaunchForward(Forward a, int32_t x_type, int32_t y_type, LaunchOn on) {
-    if (x_type == MGT_F32 && y_type == MGT_F32) RunTyped<float, float>(a, x_type, y_type, on);
-    else if (x_type == MGT_F32 && y_type == MGT_F16) RunTyped<float, __half>(a, x_type, y_type, on);
-    else if (x_type == MGT_F32 && y_type == MGT_BF16) RunTyped<float, __nv_bfloat16>(a, x_type, y_type, on);
-    else if (x_type == MGT_F16 && y_type == MGT_F16) RunTyped<__half, __half>(a, x_type, y_type, on);
-    else if (x_type == MGT_F16 && y_type == MGT_F32) RunTyped<__half, float>(a, x_type, y_type, on);
-    else if (x_type == MGT_BF16 && y_type == MGT_BF16) RunTyped<__nv_bfloat16, __nv_bfloat16>(a, x_type, y_type, on);
-    else if (x_type == MGT_BF16 && y_type == MGT_F32) RunTyped<__nv_bfloat16, float>(a, x_type, y_type, on);
-    else return MGT_INVALID_CONFIG;
-    return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
+    if (x_type == MGT_F32 && y_type == MGT_F32) return RunTyped<float, float>(a, x_type, y_type, on);
+    if (x_type == MGT_F32 && y_type == MGT_F16) return RunTyped<float, __half>(a, x_type, y_type, on);
+    if (x_type == MGT_F32 && y_type == MGT_BF16) return RunTyped<float, __nv_bfloat16>(a, x_type, y_type, on);
+    if (x_type == MGT_F16 && y_type == MGT_F16) return RunTyped<__half, __half>(a, x_type, y_type, on);
+    if (x_type == MGT_F16 && y_type == MGT_F32) return RunTyped<__half, float>(a, x_type, y_type, on);
+    if (x_type == MGT_BF16 && y_type == MGT_BF16) return RunTyped<__nv_bfloat16, __nv_bfloat16>(a, x_type, y_type, on);
+    if (x_type == MGT_BF16 && y_type == MGT_F32) return RunTyped<__nv_bfloat16, float>(a, x_type, y_type, on);
+    return MGT_INVALID_CONFIG;
 }
 
 mgt_status_t LaunchTowerForward(Forward a, bool bf16, LaunchOn on) {
-    const Cut cut = CutRow(a.cols, 4, 16);  // widths of a tower: a warp a row at most
-    if (cut.lanes > 32U || cut.stream) return MGT_INVALID_CONFIG;
+    const uint32_t v = a.cols % 4U == 0 && a.x_pitch % 4U == 0 && a.y_pitch % 4U == 0 ? 4U : 1U;
+    const Cut cut = CutRow(a.rows, a.cols, v);
+    if (cut.threads > 256U || cut.stream) return MGT_INVALID_CONFIG;  // (no tower is that wide)
     auto run = [&](auto type) {
         using T = decltype(type);
-        if (cut.nv == 1) Run<float, T, 4, 1, 256, true>(a, cut, on);
-        else if (cut.nv == 2) Run<float, T, 4, 2, 256, true>(a, cut, on);
-        else Run<float, T, 4, 4, 256, true>(a, cut, on);
+        if (v == 1U) return cut.nv <= 4 ? Run<float, T, 1, 4, 256, true>(a, cut, on) : Run<float, T, 1, 16, 256, true>(a, cut, on);
+        if (cut.nv == 1) return Run<float, T, 4, 1, 256, true>(a, cut, on);
+        if (cut.nv == 2) return Run<float, T, 4, 2, 256, true>(a, cut, on);
+        return Run<float, T, 4, 4, 256, true>(a, cut, on);
     };
-    if (bf16) run(__nv_bfloat16{}); else run(__half{});
-    return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
+    return bf16 ? run(__nv_bfloat16{}) : run(__half{});
 }
 
 }  // namespace ln

@@ -68,8 +68,7 @@ def test_host_tensors_are_refused():
     if torch.cuda.is_available():
         pytest.skip("for machines without a device: here the current device is asked for")
     cfg = mgt.LayerNormConfig(4, 8)
-    with pytest.raises(Exception):  # no device to be current
-        mgt.launch_layer_norm(cfg, torch.zeros(4, 8), None, None, torch.zeros(4, 8), stream=0)
+    assert mgt.launch_layer_norm(cfg, torch.zeros(4, 8), None, None, torch.zeros(4, 8), stream=0) == 1
     with pytest.raises(mgt.MgtError):
         mgt.TensorList([torch.zeros(4)])
     with pytest.raises(mgt.MgtError):
