@@ -148,18 +148,23 @@ ChunkSquaresKernel(const __grid_constant__ Table<kMost> t, double* __restrict__ 
     }
 }
 
-// result = {norm, scale}; norms: of every tensor, if wanted.
+// result = {norm, scale}; norms: of every tensor, if wanted. The chunks' sums come to shared memory at once, all loads in flight together; a
+// tensor's are then added by the lanes of a warp, and the tensors by the CTA.
 template <uint32_t kMost>
 __global__ void __launch_bounds__(kFinishThreads)
 FinishNormKernel(const __grid_constant__ Table<kMost> t, const double* __restrict__ partial, float max_norm, float* __restrict__ result, float* __restrict__ norms) {
-    __shared__ double squares[kMost];
-    __shared__ double warps[kFinishThreads / 32U];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31U;
+    __shared__ double chunks[kWantedChunks + kMost], squares[kMost], warps[kFinishThreads / 32U];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31U, all = t.first_chunk[t.tensors];
     mgt::dependent_begin();
+#pragma unroll
+    for (uint32_t c = threadIdx.x; c < kWantedChunks + kMost; c += kFinishThreads)
+        if (c < all) chunks[c] = partial[c];
+    __syncthreads();
     for (uint32_t k = warp; k < t.tensors; k += kFinishThreads / 32U) {
+        const uint32_t end = t.first_chunk[k + 1U];
         double s = 0.0;
 #pragma unroll 4
-        for (uint32_t c = t.first_chunk[k] + lane; c < t.first_chunk[k + 1U]; c += 32U) s += partial[c];
+        for (uint32_t c = t.first_chunk[k] + lane; c < end; c += 32U) s += chunks[c];
         s = WarpSum(s);
         if (lane == 0U) {
             squares[k] = s;

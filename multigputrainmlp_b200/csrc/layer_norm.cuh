@@ -1,5 +1,5 @@
 // Layer normalisation: how rows are held and fetched. A row of C columns is shared by `lanes` threads (a power of two, at most a CTA); thread
-// t has the packs t, t + lanes, ... of V neighbouring elements, at most 16 elements in all. Several rows lie side by side in a CTA. Groups
+// t has the packs t, t + lanes, ... of V neighbouring elements, 16 elements at most. Several rows lie side by side in a CTA. Groups
 // of up to 32 lanes reduce by shuffles, wider ones through shared memory and a barrier of their own.
 //
 // The kernels are bound by HBM, and what that takes is bytes in flight: some 45 KB an SM at 6.5 TB/s and a loaded latency of 1 us. One
@@ -51,18 +51,28 @@ __device__ __forceinline__ void StorePack(T* p, const Pack<T, V>& v) {
 // single values, and instructions are what bounds these kernels once their loads are far enough ahead.
 __device__ __forceinline__ uint64_t& Bits(float2& v) { return reinterpret_cast<uint64_t&>(v); }
 __device__ __forceinline__ float2 Add2(float2 a, float2 b) {
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(Bits(a)) : "l"(Bits(b)));
-    return a;
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(Bits(r)) : "l"(Bits(a)), "l"(Bits(b)));
+    return r;
 }
 __device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
-    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(Bits(a)) : "l"(Bits(b)));
-    return a;
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(Bits(r)) : "l"(Bits(a)), "l"(Bits(b)));
+    return r;
 }
 __device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(Bits(c)) : "l"(Bits(a)), "l"(Bits(b)));
-    return c;
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(Bits(r)) : "l"(Bits(a)), "l"(Bits(b)), "l"(Bits(c)));
+    return r;
 }
 __device__ __forceinline__ float2 Both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 Up(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 Up(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ float2 Up(float2 v) { return v; }
+template <class T> struct Two;
+template <> struct Two<float> { using type = float2; static __device__ __forceinline__ float2 Down(float2 v) { return v; } };
+template <> struct Two<__half> { using type = __half2; static __device__ __forceinline__ __half2 Down(float2 v) { return __floats2half2_rn(v.x, v.y); } };
+template <> struct Two<__nv_bfloat16> { using type = __nv_bfloat162; static __device__ __forceinline__ __nv_bfloat162 Down(float2 v) { return __floats2bfloat162_rn(v.x, v.y); } };
 template <int E>
 struct Held {
     static constexpr int kPairs = (E + 1) / 2;
@@ -78,37 +88,57 @@ struct Held {
 // with it everybody's reads of this one.
 struct Group {
     uint32_t lanes, lane, index, count;  // threads of a group, place in it, group of the CTA, groups of the CTA
-    float2* buffer;                      // [2][warps of the CTA]
+    float* buffer;                       // [2][warps of the CTA][values of a reduction]
     uint32_t turn;
 };
-__device__ __forceinline__ Group MakeGroup(uint32_t lanes, float2* buffer) {
+__device__ __forceinline__ Group MakeGroup(uint32_t lanes, float* buffer) {
     return {lanes, threadIdx.x & (lanes - 1U), threadIdx.x / lanes, blockDim.x / lanes, buffer, 0U};
 }
-// Sums of one or two values over the group, in every one of its threads. All threads of a warp come here together.
+// Sums of N values (a power of two) over the group, in every one of its threads. All threads of a warp come here together. Groups of N lanes
+// and more halve the values that a lane still adds up with every step, N - 1 shuffles for the first log2(N) of them instead of N log2(N).
+constexpr __host__ __device__ int ReverseBits(int i, int n) { return n <= 1 ? 0 : (i & 1) * (n / 2) + ReverseBits(i / 2, n / 2); }
 template <int N>
 __device__ __forceinline__ void Reduce(Group& g, float (&v)[N]) {
+    const uint32_t lane = threadIdx.x & 31U;
+    if (g.lanes < N) {
 #pragma unroll
-    for (uint32_t o = 16U; o > 0U; o >>= 1) {
-        if (o >= g.lanes) continue;  // (the same for the whole CTA)
-#pragma unroll
-        for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffU, v[n], o);
-    }
-    if (g.lanes > 32U) {
-        const uint32_t warps = g.lanes >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31U;
-        float2* at = g.buffer + (g.turn & 1U) * (blockDim.x >> 5);
-        g.turn ^= 1U;
-        if (lane == 0U) at[warp] = make_float2(v[0], v[N - 1]);
-        asm volatile("bar.sync %0, %1;" ::"r"(1U + g.index), "r"(g.lanes) : "memory");
-        const float2 part = at[g.index * warps + (lane & (warps - 1U))];  // (each of them in 32 / warps lanes: no broadcast behind the tree)
-        v[0] = part.x;
-        v[N - 1] = N > 1 ? part.y : part.x;
-#pragma unroll
-        for (uint32_t o = 16U; o > 0U; o >>= 1) {
-            if (o >= warps) continue;
+        for (uint32_t o = N / 2U; o > 0U; o >>= 1) {
+            if (o >= g.lanes) continue;  // (the same for the whole CTA)
 #pragma unroll
             for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffU, v[n], o);
         }
+        return;
     }
+#pragma unroll
+    for (int half = N / 2; half > 0; half /= 2) {  // lanes with the step's bit keep the upper half
+        const int o = N / 2 / half;
+        const bool up = (lane & o) != 0U;
+#pragma unroll
+        for (int n = 0; n < half; ++n) {
+            const float give = up ? v[n] : v[n + half], keep = up ? v[n + half] : v[n];
+            v[n] = keep + __shfl_xor_sync(0xffffffffU, give, o);
+        }
+    }
+    float mine = v[0];  // of value ReverseBits(lane % N)
+#pragma unroll
+    for (uint32_t o = N; o < 32U; o <<= 1)
+        if (o < g.lanes) mine += __shfl_xor_sync(0xffffffffU, mine, o);
+    if (g.lanes > 32U) {
+        const uint32_t warps = g.lanes >> 5, warp = threadIdx.x >> 5;
+        float* at = g.buffer + (g.turn & 1U) * (blockDim.x >> 5) * N;
+        g.turn ^= 1U;
+        if (lane < N) at[warp * N + lane] = mine;
+        asm volatile("bar.sync %0, %1;" ::"r"(1U + g.index), "r"(g.lanes) : "memory");
+        mine = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < 32U; w += 32U / N)
+            if (w + lane / N < warps) mine += at[(g.index * warps + w) * N + lane];
+#pragma unroll
+        for (uint32_t o = N; o < 32U; o <<= 1) mine += __shfl_xor_sync(0xffffffffU, mine, o);
+    }
+    const uint32_t base = g.lanes < 32U ? lane & ~(g.lanes - 1U) : 0U;
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = N == 1 ? mine : __shfl_sync(0xffffffffU, mine, base + ReverseBits(n, N));
 }
 
 // Which rows a group has: the first one, every stride-th from there, `mine` in all; `turns` of the warp's group that has most.
@@ -169,49 +199,67 @@ struct Ring {
         if constexpr (V > 1) return slots + (turn * NV + i) * (kThreads * kPackBytes);
         else return slots + turn * g.count * line_bytes;
     }
+    // The group's next row, zeros where there is none left.
     __device__ __forceinline__ void Fetch(const Group& g, uint32_t turn, bool in) {
-        if (in) {
-            if constexpr (V > 1) {
+        if constexpr (V > 1) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (PackColumn<V>(g, i) < cols) CopyAsync<kPackBytes>(static_cast<uint32_t>(__cvta_generic_to_shared(Slot(g, turn, i))), next + i * g.lanes * V);
-            } else {
-                const uintptr_t begin = reinterpret_cast<uintptr_t>(next), end = begin + static_cast<uintptr_t>(cols) * sizeof(T);
-                char* to = Slot(g, turn, 0) + 16U * g.lane;
-                for (uintptr_t line = (begin & ~static_cast<uintptr_t>(15)) + 16U * g.lane; line < end; line += 16U * g.lanes, to += 16U * g.lanes) {
-                    if (line >= least && line + 16U <= most) {
-                        CopyAsync<16>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), reinterpret_cast<const void*>(line));
-                    } else {
-                        for (uintptr_t e = line < begin ? begin : line; e < end && e < line + 16U; e += sizeof(T))
-                            *reinterpret_cast<T*>(to + (e - line)) = *reinterpret_cast<const T*>(e);
-                    }
+            for (int i = 0; i < NV; ++i) {
+                if (PackColumn<V>(g, i) >= cols) continue;
+                if (in) CopyAsync<kPackBytes>(static_cast<uint32_t>(__cvta_generic_to_shared(Slot(g, turn, i))), next + i * g.lanes * V);
+                else *reinterpret_cast<typename Word<kPackBytes>::type*>(Slot(g, turn, i)) = {};
+            }
+        } else if (in) {
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(next), end = begin + static_cast<uintptr_t>(cols) * sizeof(T);
+            char* to = Slot(g, turn, 0) + 16U * g.lane;
+            for (uintptr_t line = (begin & ~static_cast<uintptr_t>(15)) + 16U * g.lane; line < end; line += 16U * g.lanes, to += 16U * g.lanes) {
+                if (line >= least && line + 16U <= most) {
+                    CopyAsync<16>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), reinterpret_cast<const void*>(line));
+                } else {
+                    for (uintptr_t e = line < begin ? begin : line; e < end && e < line + 16U; e += sizeof(T))
+                        *reinterpret_cast<T*>(to + (e - line)) = *reinterpret_cast<const T*>(e);
                 }
             }
         }
         next += step;
     }
+    // Before the first fetch: what lies beyond the row's end is zero in every slot and stays so (V > 1).
+    __device__ __forceinline__ void Clear(const Group& g) {
+        if constexpr (V > 1) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (PackColumn<V>(g, i) >= cols)
+                    for (uint32_t turn = 0; turn < kDepth; ++turn) *reinterpret_cast<typename Word<kPackBytes>::type*>(Slot(g, turn, i)) = {};
+        }
+    }
     // This thread's elements of a row that has arrived; zeros beyond the row's end, and where there is no row.
     __device__ __forceinline__ void Read(Held<NV * V>& out, const Group& g, uint32_t turn, bool in) {
-        const char* line = V > 1 ? nullptr : Slot(g, turn, 0) + (reinterpret_cast<uintptr_t>(now) & 15U);
+        if constexpr (V > 1) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i);
-            const T* from = V > 1 ? reinterpret_cast<const T*>(Slot(g, turn, i)) : reinterpret_cast<const T*>(line) + c;
-            Pack<T, V> p;
-            using W = typename Word<kPackBytes>::type;
-            *reinterpret_cast<W*>(&p) = W{};
-            if (in && c < cols) p = LoadPack<T, V>(from);
+            for (int i = 0; i < NV; ++i) {
+                const Pack<T, V> p = LoadPack<T, V>(reinterpret_cast<const T*>(Slot(g, turn, i)));
 #pragma unroll
-            for (int j = 0; j < V; ++j) out.Set(i * V + j, ToFloat(p.v[j]));
+                for (int j = 0; j < V / 2; ++j) out.pair[i * (V / 2) + j] = Up(reinterpret_cast<const typename Two<T>::type*>(&p)[j]);
+            }
+        } else {
+            const T* line = reinterpret_cast<const T*>(Slot(g, turn, 0) + (reinterpret_cast<uintptr_t>(now) & 15U));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t c = PackColumn<V>(g, i);
+                out.Set(i, in && c < cols ? ToFloat(line[c]) : 0.0f);
+            }
+            now += step;
         }
-        now += step;
     }
 };
 template <class T, int V, int E>
 __device__ __forceinline__ Pack<T, V> PackOf(const Held<E>& v, int i) {
     Pack<T, V> p;
+    if constexpr (V == 1) {
+        p.v[0] = FromFloat<T>(v.Get(i));
+    } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) p.v[j] = FromFloat<T>(v.Get(i * V + j));
+        for (int j = 0; j < V / 2; ++j) reinterpret_cast<typename Two<T>::type*>(&p)[j] = Two<T>::Down(v.pair[i * (V / 2) + j]);
+    }
     return p;
 }
 // `value` where the thread's elements are in the row, zero where they are not.

@@ -9,27 +9,39 @@ namespace ln {
 namespace {
 
 constexpr uint32_t kSums = 3;
-constexpr uint32_t kMostCtas = 296;     // partial rows at most: two CTAs on each of 148 SMs
+constexpr uint32_t kSms = 148, kMostCtas = 2 * kSms;  // partial rows at most: two CTAs an SM
 constexpr int kMostShared = 200 << 10;
 constexpr uint32_t kColumnSlices = 37;  // widest rows: slices of the batch that the column sums are taken over
 
-template <class Tdy, class Tx, int V, int NV>
-constexpr int kDepth = V == 1 ? 2 : NV * V * (sizeof(Tdy) + sizeof(Tx)) >= 64 ? 3 : 6;
+inline __host__ __device__ uint32_t PartialPitch(uint32_t cols) { return (cols + 3U) / 4U * 4U; }
 
-template <class Tdy, class Tx, class Tdx, int V, int NV, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
+// What a kernel is made of: packs of a thread, threads, rows on their way, CTAs an SM.
+template <class Tdy, class Tx, int V_, int NV_, int kThreads_>
+struct Form {
+    static constexpr int V = V_, NV = NV_, kThreads = kThreads_, E = V * NV;
+    static constexpr int kBytes = E * (sizeof(Tdy) + sizeof(Tx)) * kThreads;  // of a row of every group
+    static constexpr int kDepth = V == 1 || kBytes > (32 << 10) ? 2 : kBytes >= (16 << 10) ? 3 : 6;
+    static constexpr int kCtas = kThreads > 256 ? 1 : 2;
+    using RingDy = Ring<Tdy, V, NV, kThreads, kDepth>;
+    using RingX = Ring<Tx, V, NV, kThreads, kDepth>;
+    static constexpr uint32_t kGammaBytes = E * kThreads * 4U;
+};
+
+template <class Tdy, class Tx, class Tdx, class F>
+__global__ void __launch_bounds__(F::kThreads, F::kCtas)
 BackwardKernel(const Backward a) {
-    extern __shared__ __align__(16) char memory[];  // the rings; at the end [groups][cols] sums, where there is more than one group
-    __shared__ float2 buffer[2 * (kThreads / 32)];
-    constexpr int D = kDepth<Tdy, Tx, V, NV>, kPairs = Held<NV * V>::kPairs;
-    using RingDy = Ring<Tdy, V, NV, kThreads, D>;
+    extern __shared__ __align__(16) char memory[];  // gamma, the rings; at the end [groups][cols] sums, where there is more than one group
+    constexpr int V = F::V, NV = F::NV, E = F::E, D = F::kDepth, kThreads = F::kThreads, kPairs = Held<E>::kPairs;
+    __shared__ float buffer[2 * 2 * (kThreads / 32)];
     Group g = MakeGroup(a.lanes, buffer);
     const Share share = MakeShare(g, a.rows);
-    RingDy ring_dy(a.dy, a.dy_pitch, a.rows, a.cols, memory, g, share);
-    Ring<Tx, V, NV, kThreads, D> ring_x(a.x, a.x_pitch, a.rows, a.cols, memory + RingDy::Bytes(a.cols, g.count), g, share);
+    typename F::RingDy ring_dy(a.dy, a.dy_pitch, a.rows, a.cols, memory + F::kGammaBytes, g, share);
+    typename F::RingX ring_x(a.x, a.x_pitch, a.rows, a.cols, memory + F::kGammaBytes + F::RingDy::Bytes(a.cols, g.count), g, share);
     const float per_col = 1.0f / static_cast<float>(a.cols);
     Tdx* dx = static_cast<Tdx*>(a.dx) + share.first * a.dx_pitch + g.lane * V;
     const uint64_t dx_step = share.stride * a.dx_pitch;
+    ring_dy.Clear(g);
+    ring_x.Clear(g);
     dependent_begin();
 #pragma unroll
     for (int d = 0; d < D; ++d) {
@@ -37,36 +49,44 @@ BackwardKernel(const Backward a) {
         ring_x.Fetch(g, d, d < share.mine);
         CopiesEnd();
     }
-    float next_mean = 0.0f, next_rstd = 0.0f;
-    if (share.mine != 0U) {
-        next_mean = a.mean[share.first];
-        next_rstd = a.rstd[share.first];
-    }
-    Held<NV * V> gamma, sums[kSums], gy, xhat;
+    float next_mean, next_rstd;
+    const float* mean_at = a.mean + share.first;
+    const float* rstd_at = a.rstd + share.first;
+    auto load_statistics = [&](uint32_t t) {  // (a row that is not there adds nothing to the sums)
+        next_mean = t < share.mine ? *mean_at : 0.0f;
+        next_rstd = t < share.mine ? *rstd_at : 0.0f;
+        mean_at += share.stride;
+        rstd_at += share.stride;
+    };
+    load_statistics(0);
+    float4* gamma_at = reinterpret_cast<float4*>(memory) + threadIdx.x;  // this thread's columns: in registers they would spill beside the sums
+    Held<E> gy, xhat, gamma, sums[kSums];
     LoadColumns<V, NV>(gamma, g, a.cols, a.gamma, 1.0f);
+#pragma unroll
+    for (int k = 0; k < E; k += 4) gamma_at[k / 4 * kThreads] = make_float4(gamma.Get(k), gamma.Get(k + 1), gamma.Get(k + 2), gamma.Get(k + 3));
 #pragma unroll
     for (uint32_t n = 0; n < kSums; ++n)
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) sums[n].pair[k] = Both(0.0f);
-    uint32_t slot = 0, row = share.first;
+    uint32_t slot = 0;
     for (uint32_t t = 0; t < share.turns; ++t) {
         const bool in = t < share.mine;
-        const float mean = in ? next_mean : 0.0f, rstd = in ? next_rstd : 0.0f;  // (a row that is not there adds nothing to the sums)
-        row += share.stride;
-        if (t + 1U < share.mine) {
-            next_mean = a.mean[row];
-            next_rstd = a.rstd[row];
-        }
+        const float2 less = Both(-next_mean), rstd = Both(next_rstd);
+        load_statistics(t + 1U);
         CopiesWait<D - 1>();
         if (V == 1) GroupBarrier(g);
         ring_dy.Read(gy, g, slot, in);
         ring_x.Read(xhat, g, slot, in);
-        Held<NV * V> less;
-        InRow<V, NV>(less, g, a.cols, -mean);
+#pragma unroll
+        for (int k = 0; k < E; k += 4) {
+            const float4 q = gamma_at[k / 4 * kThreads];
+            gamma.pair[k / 2] = make_float2(q.x, q.y);
+            gamma.pair[k / 2 + 1] = make_float2(q.z, q.w);
+        }
         float2 s1 = Both(0.0f), s2 = Both(0.0f);
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-            xhat.pair[k] = Mul2(Add2(xhat.pair[k], less.pair[k]), Both(rstd));
+        for (int k = 0; k < kPairs; ++k) {  // (beyond the row's end dy is zero, and with it all that xhat enters)
+            xhat.pair[k] = Mul2(Add2(xhat.pair[k], less), rstd);
             sums[0].pair[k] = Fma2(gy.pair[k], xhat.pair[k], sums[0].pair[k]);
             sums[1].pair[k] = Add2(gy.pair[k], sums[1].pair[k]);
             gy.pair[k] = Mul2(gy.pair[k], gamma.pair[k]);
@@ -81,10 +101,10 @@ BackwardKernel(const Backward a) {
         CopiesEnd();
         slot = slot + 1U == D ? 0U : slot + 1U;
         if (in) {
-            const float2 c1 = Both(-s[0] * per_col), c2 = Both(-s[1] * per_col), scale = Both(rstd);
+            const float2 c1 = Both(-s[0] * per_col), c2 = Both(-s[1] * per_col);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) {
-                gy.pair[k] = Mul2(scale, Fma2(xhat.pair[k], c2, Add2(gy.pair[k], c1)));  // (rstd last: it is large where the differences are small)
+                gy.pair[k] = Mul2(rstd, Fma2(xhat.pair[k], c2, Add2(gy.pair[k], c1)));  // (rstd last: it is large where the differences are small)
                 sums[2].pair[k] = Add2(gy.pair[k], sums[2].pair[k]);  // (before it is rounded to dx's type; beyond the row's end nobody looks)
             }
 #pragma unroll
@@ -97,11 +117,12 @@ BackwardKernel(const Backward a) {
     float* lanes_sums = reinterpret_cast<float*>(memory);
     __syncthreads();  // (the rings are no longer read)
     // this CTA's column sums: the groups in order
-    float* partial = a.partial + static_cast<uint64_t>(blockIdx.x) * kSums * a.cols;
+    const uint32_t pitch = PartialPitch(a.cols);
+    float* partial = a.partial + static_cast<uint64_t>(blockIdx.x) * kSums * pitch;
 #pragma unroll
     for (uint32_t k = 0; k < kSums; ++k) {
         if (a.sums[k] == nullptr) continue;
-        float* to = gridDim.x > 1U ? partial + k * a.cols : a.sums[k];
+        float* to = gridDim.x > 1U ? partial + k * pitch : a.sums[k];
         float* mine = g.count > 1U ? lanes_sums + g.index * a.cols : to;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -122,36 +143,41 @@ BackwardKernel(const Backward a) {
     }
 }
 
-// sums[k][c] = the partial rows' values added up: 64 threads share a column, each adds every 64th row in order, then a binary tree.
-constexpr uint32_t kSumCols = 16, kSumParts = 64;
-__global__ void __launch_bounds__(kSumCols * kSumParts)
-SumPartialRowsKernel(const Backward a, uint32_t rows) {
-    __shared__ float part_sums[kSumParts][kSumCols];
-    const uint32_t c = threadIdx.x % kSumCols, part = threadIdx.x / kSumCols, col = blockIdx.x * kSumCols + c;
+// sums[k][c] = the partial rows' values added up: 32 threads share four neighbouring columns, each adds every 32nd row in order (ten loads in
+// flight at most: one trip to L2), and the 32 then in order. Rows of partial sums are whole quads apart; what lies behind the last column is read and not used.
+constexpr uint32_t kSumQuads = 8, kSumParts = 32;
+__global__ void __launch_bounds__(kSumQuads * kSumParts)
+SumPartialRowsKernel(const Backward a, uint32_t rows, uint32_t pitch) {
+    __shared__ float4 part_sums[kSumParts][kSumQuads];
+    const uint32_t q = threadIdx.x % kSumQuads, part = threadIdx.x / kSumQuads, quad = blockIdx.x * kSumQuads + q;
     dependent_begin();
     float* to = a.sums[blockIdx.y];
     if (to == nullptr) return;
-    float s = 0.0f;
-    if (col < a.cols) {
-        const float* from = a.partial + static_cast<uint64_t>(blockIdx.y) * a.cols + col;
-#pragma unroll 5
-        for (uint32_t r = part; r < rows; r += kSumParts) s += from[static_cast<uint64_t>(r) * kSums * a.cols];
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (quad * 4U < a.cols) {
+        const float4* from = reinterpret_cast<const float4*>(a.partial + blockIdx.y * pitch) + quad;
+        const uint64_t step = kSums * (pitch / 4U);
+#pragma unroll 10
+        for (uint32_t r = part; r < rows; r += kSumParts) {
+            const float4 v = from[r * step];
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
     }
-    part_sums[part][c] = s;
+    part_sums[part][q] = s;
     __syncthreads();
+    const uint32_t col = blockIdx.x * kSumQuads * 4U + threadIdx.x;
+    if (threadIdx.x < kSumQuads * 4U && col < a.cols) {
+        float total = 0.0f;
 #pragma unroll
-    for (uint32_t half = kSumParts / 2U; half > 0U; half >>= 1) {
-        if (part < half) part_sums[part][c] += part_sums[part + half][c];
-        __syncthreads();
+        for (uint32_t p = 0; p < kSumParts; ++p) total += reinterpret_cast<const float*>(part_sums[p])[threadIdx.x];
+        to[col] = total;
     }
-    if (part == 0U && col < a.cols) to[col] = part_sums[0][c];
 }
-
 // Rows wider than the registers of a CTA. First the two means of every row, left in `means` ...
 template <class Tdy, class Tx, int V>
 __global__ void __launch_bounds__(1024)
 StreamMeansKernel(const Backward a, float2* means) {
-    __shared__ float2 buffer[2 * 32];
+    __shared__ float buffer[2 * 2 * 32];
     Group g = MakeGroup(blockDim.x, buffer);
     const float cols = static_cast<float>(a.cols);
     const uint32_t step = blockDim.x * V;
@@ -204,31 +230,30 @@ StreamColumnsKernel(const Backward a, const float2* means, uint32_t rows_each) {
         }
         StorePack<Tdx, V>(static_cast<Tdx*>(a.dx) + row * a.dx_pitch + c, out);
     }
-    float* partial = a.partial + static_cast<uint64_t>(blockIdx.y) * kSums * a.cols;
+    const uint32_t pitch = PartialPitch(a.cols);
+    float* partial = a.partial + static_cast<uint64_t>(blockIdx.y) * kSums * pitch;
 #pragma unroll
     for (uint32_t k = 0; k < kSums; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) partial[k * a.cols + c + j] = sums[k][j];
+        for (int j = 0; j < V; ++j) partial[k * pitch + c + j] = sums[k][j];
 }
 
 void SumPartialRows(const Backward& a, uint32_t rows, LaunchOn on, uint32_t* launches) {
-    Launch(SumPartialRowsKernel, dim3((a.cols + kSumCols - 1U) / kSumCols, kSums), kSumCols * kSumParts, 0, LaunchOn(on.stream, true), a, rows);
+    Launch(SumPartialRowsKernel, dim3((a.cols + 4U * kSumQuads - 1U) / (4U * kSumQuads), kSums), kSumQuads * kSumParts, 0, LaunchOn(on.stream, true), a, rows, PartialPitch(a.cols));
     ++*launches;
 }
 
-template <class Tdy, class Tx, class Tdx, int V, int NV, int kThreads>
+template <class Tdy, class Tx, class Tdx, class F>
 mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint32_t groups = cut.threads / cut.lanes;
     const uint64_t want = (static_cast<uint64_t>(a.rows) + groups - 1U) / groups;
-    const uint32_t most = cut.threads == 256U ? kMostCtas : kMostCtas / 2U;
-    const uint32_t ctas = static_cast<uint32_t>(want < most ? want : most);
+    const uint32_t most = kSms * F::kCtas, ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
-    constexpr int D = kDepth<Tdy, Tx, V, NV>;
-    const uint32_t rings = Ring<Tdy, V, NV, kThreads, D>::Bytes(a.cols, groups) + Ring<Tx, V, NV, kThreads, D>::Bytes(a.cols, groups);
+    const uint32_t rings = F::kGammaBytes + F::RingDy::Bytes(a.cols, groups) + F::RingX::Bytes(a.cols, groups);
     const uint32_t sums = groups > 1U ? groups * a.cols * 4U : 0U, smem = rings > sums ? rings : sums;
     static std::atomic<uint64_t> allowed{0};
-    if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, V, NV, kThreads>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
-    Launch(BackwardKernel<Tdy, Tx, Tdx, V, NV, kThreads>, ctas, cut.threads, smem, on, a);
+    if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, F>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
+    Launch(BackwardKernel<Tdy, Tx, Tdx, F>, ctas, cut.threads, smem, on, a);
     ++*launches;
     if (ctas > 1U && (a.sums[0] != nullptr || a.sums[1] != nullptr || a.sums[2] != nullptr)) SumPartialRows(a, ctas, on, launches);
     return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
@@ -237,8 +262,8 @@ template <class Tdy, class Tx, class Tdx, int V>
 mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
     const Cut cut = CutRow(a.rows, a.cols, V);
     if (cut.stream) {
-        float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kMostCtas) * kSums * a.cols);
-        Launch(StreamMeansKernel<Tdy, Tx, V>, a.rows < 296U ? a.rows : 296U, 1024, 0, on, a, means);
+        float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(a.cols));
+        Launch(StreamMeansKernel<Tdy, Tx, V>, a.rows < 2U * kSms ? a.rows : 2U * kSms, 1024, 0, on, a, means);
         const uint32_t slices = a.rows < kColumnSlices ? a.rows : kColumnSlices, rows_each = (a.rows - 1U) / slices + 1U;
         const uint32_t used = (a.rows - 1U) / rows_each + 1U;
         Launch(StreamColumnsKernel<Tdy, Tx, Tdx, V>, dim3((a.cols - 1U) / (256U * V) + 1U, used), 256, 0, LaunchOn(on.stream, true), a, static_cast<const float2*>(means), rows_each);
@@ -246,11 +271,11 @@ mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
         SumPartialRows(a, used, on, launches);
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
-    constexpr int kMost = kElements / V, kFew = V == 1 ? 4 : 2;  // packs a thread that there are kernels for, besides one
-    if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, V, kMost, 512>(a, cut, on, launches);
-    if (cut.nv == 1) return Run<Tdy, Tx, Tdx, V, 1, 256>(a, cut, on, launches);
-    if (cut.nv <= kFew) return Run<Tdy, Tx, Tdx, V, kFew, 256>(a, cut, on, launches);
-    return Run<Tdy, Tx, Tdx, V, kMost, 256>(a, cut, on, launches);
+    // (packs that the kernel has room for and the row does not have lie beyond its end)
+    constexpr int kMost = kElements / V, kFew = V == 1 ? 4 : V == 4 ? 2 : 1;
+    if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, V, kMost, 512>>(a, cut, on, launches);
+    if (cut.nv <= kFew) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, V, kFew, 256>>(a, cut, on, launches);
+    return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, V, kMost, 256>>(a, cut, on, launches);
 }
 template <class Tdy, class Tx, class Tdx>
 mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {
@@ -267,7 +292,7 @@ mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_
 }  // namespace
 
 uint64_t BackwardFloats(uint32_t rows, uint32_t cols) {
-    return static_cast<uint64_t>(kMostCtas) * kSums * cols + (cols > kElements * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
+    return static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(cols) + (cols > kElements * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
 }
 
 mgt_status_t LaunchBackward(Backward a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {
@@ -314,7 +339,7 @@ mgt_status_t mgt_launch_layer_norm_backward(const mgt_layer_norm_config_t* c, co
     mgt::ln::Backward a{};
     a.dy = dy; a.x = x; a.dx = dx; a.gamma = gamma; a.mean = mean; a.rstd = rstd;
     for (int k = 0; k < 3; ++k) a.sums[k] = sums[k];
-    a.partial = workspace;
+    a.partial = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15U) & ~static_cast<uintptr_t>(15));
     a.dy_pitch = c->y_pitch != 0 ? c->y_pitch : c->cols;
     a.x_pitch = c->x_pitch != 0 ? c->x_pitch : c->cols;
     a.dx_pitch = c->dx_pitch != 0 ? c->dx_pitch : c->cols;

@@ -27,7 +27,7 @@ template <class Tx, class Ty, int V, int NV, int kThreads, bool kTower>
 __global__ void __launch_bounds__(kThreads, kThreads == 256 ? kCtasPerSm : 1)
 ForwardKernel(const Forward a) {
     extern __shared__ __align__(16) char memory[];
-    __shared__ float2 buffer[2 * (kThreads / 32)];
+    __shared__ float buffer[2 * 2 * (kThreads / 32)];
     constexpr int D = kDepth<Tx, V, NV>, kPairs = Held<NV * V>::kPairs;
     Group g = MakeGroup(a.lanes, buffer);
     const Share share = MakeShare(g, a.rows);
@@ -36,6 +36,7 @@ ForwardKernel(const Forward a) {
     Ty* y = static_cast<Ty*>(a.y) + share.first * a.y_pitch + g.lane * V;
     float* state = kTower ? a.state + share.first * a.x_pitch + g.lane * V : nullptr;
     const uint64_t y_step = share.stride * a.y_pitch, state_step = share.stride * a.x_pitch;
+    ring.Clear(g);
     dependent_begin();
 #pragma unroll
     for (int d = 0; d < D; ++d) {
@@ -100,7 +101,7 @@ ForwardKernel(const Forward a) {
 template <class Tx, class Ty, int V>
 __global__ void __launch_bounds__(1024)
 StreamForwardKernel(const Forward a) {
-    __shared__ float2 buffer[2 * 32];
+    __shared__ float buffer[2 * 2 * 32];
     Group g = MakeGroup(blockDim.x, buffer);
     const float per_col = 1.0f / static_cast<float>(a.cols);
     const uint32_t step = blockDim.x * V;
