@@ -155,9 +155,38 @@ __device__ __forceinline__ Share MakeShare(const Group& g, uint32_t rows) {
     return s;
 }
 
-// Column of this thread's pack i. Packs are whole: the row has all of one or nothing.
-template <int V>
-__device__ __forceinline__ uint32_t PackColumn(const Group& g, int i) { return (static_cast<uint32_t>(i) * g.lanes + g.lane) * V; }
+// Which columns a thread has.
+//   V > 1   packs t, t + lanes, ... of V columns; a pack is whole: the row has all of it or nothing.
+//   V = 1   L (8 or 32) neighbouring lanes share a stretch of the row, one column to each in turn; stretches differ by a column at most. So
+//           places are constants, and only the last kMasked turns have to look at the stretch's end. (Asking at every turn took 518 instead
+//           of 230 instructions a row of 301.)
+template <int V_, int NV_, int L_, int kMasked_>
+struct Layout {
+    static constexpr int V = V_, NV = NV_, L = L_, E = V * NV, kMasked = kMasked_;
+    uint32_t cols, lanes, base;
+    uint32_t begin, end, mask;  // V = 1: the stretch, and which of the lane's last turns lie in it
+    __device__ __forceinline__ Layout(const Group& g, uint32_t cols_) : cols(cols_), lanes(g.lanes), base(g.lane * V), begin(0), end(0), mask(0) {
+        if constexpr (V == 1) {
+            const uint32_t stretch = g.lane / L, stretches = lanes / L;
+            begin = stretch * cols / stretches;
+            end = (stretch + 1U) * cols / stretches;
+            base = begin + g.lane % L;
+#pragma unroll
+            for (int i = NV - kMasked; i < NV; ++i)
+                if (base + i * L < end) mask |= 1U << i;
+        }
+    }
+    __device__ __forceinline__ uint32_t Offset(int i) const { return V > 1 ? i * lanes * V : i * L; }  // of pack i from `base`
+    __device__ __forceinline__ bool Has(int i) const {
+        if constexpr (V > 1) return base + Offset(i) < cols;
+        else return i < NV - kMasked || (mask >> i & 1U) != 0U;
+    }
+    template <class F>
+    __device__ __forceinline__ void Each(F f) const {  // f(i, whether the row has pack i)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) f(i, Has(i));
+    }
+};
 
 template <int kBytes>
 __device__ __forceinline__ void CopyAsync(uint32_t to, const void* from) {
@@ -170,84 +199,86 @@ __device__ __forceinline__ void CopiesWait() { asm volatile("cp.async.wait_group
 
 // What a thread has of its next kDepth rows of one operand, in shared memory.
 //   V > 1   packs of 16 (or 8) bytes. A thread reads only what it copied itself: nothing is shared, and nothing waits.
-//   V = 1   rows that begin anywhere: the group copies the 16-byte lines that its row lies in, and a thread reads its elements from them
-//           behind a barrier of the group. Lines that reach beyond the matrix are copied by elements.
-template <class T, int V, int NV, int kThreads, int kDepth>
+//   V = 1   rows that begin anywhere: the lanes of a stretch copy the 16-byte lines that it lies in, and read their elements from them
+//           once the warp has met. Lines that reach beyond the matrix are copied by elements.
+template <class T, class Lay, int kThreads, int kDepth>
 struct Ring {
+    static constexpr int V = Lay::V, NV = Lay::NV;
     static constexpr uint32_t kPackBytes = sizeof(T) * V;
-    const T* next;       // the row to be fetched next
-    const T* now;        // the row to be read next
-    uint64_t step;       // elements from a row of the group to its next
-    uint32_t cols, line_bytes;  // line_bytes: of a group's row (V = 1)
-    char* slots;         // of this thread (V > 1) or group
+    static constexpr uint32_t kLineBytes = (Lay::L * NV * sizeof(T) + 15U) / 16U * 16U + 16U;  // of a stretch (V = 1)
+    static constexpr uint32_t kBytes = kDepth * (V > 1 ? NV * kThreads * kPackBytes : kThreads / Lay::L * kLineBytes);
+    const T* next;              // this thread's (V > 1) or the stretch's columns in the row to be fetched next
+    uint64_t step;              // elements from a row of the group to its next
+    uint32_t now, now_step;     // where the row to be read next begins, from a 16-byte boundary (V = 1)
+    char* slots;                // of this thread (V > 1) or stretch
     uintptr_t least, most;      // the matrix (V = 1)
 
-    static __host__ __device__ uint32_t LineBytes(uint32_t cols) { return (cols * static_cast<uint32_t>(sizeof(T)) + 15U) / 16U * 16U + 16U; }
-    static __host__ __device__ uint32_t Bytes(uint32_t cols, uint32_t groups) {
-        return kDepth * (V > 1 ? NV * kThreads * kPackBytes : groups * LineBytes(cols));
-    }
-    __device__ __forceinline__ Ring(const void* base, uint64_t pitch, uint32_t rows, uint32_t cols_, char* memory, const Group& g, const Share& share) {
-        next = now = static_cast<const T*>(base) + share.first * pitch + (V > 1 ? g.lane * V : 0U);
+    __device__ __forceinline__ Ring(const void* base, uint64_t pitch, uint32_t rows, char* memory, const Share& share, const Lay& lay) {
+        next = static_cast<const T*>(base) + share.first * pitch + (V > 1 ? lay.base : lay.begin);
         step = share.stride * pitch;
-        cols = cols_;
-        line_bytes = LineBytes(cols_);
-        slots = memory + (V > 1 ? threadIdx.x * kPackBytes : g.index * line_bytes);
+        slots = memory + (V > 1 ? threadIdx.x * kPackBytes : threadIdx.x / Lay::L * kLineBytes);
+        now = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(next));
+        now_step = static_cast<uint32_t>(step * sizeof(T));
         least = reinterpret_cast<uintptr_t>(base);
-        most = reinterpret_cast<uintptr_t>(static_cast<const T*>(base) + (rows - 1ULL) * pitch + cols_);
+        most = reinterpret_cast<uintptr_t>(static_cast<const T*>(base) + (rows - 1ULL) * pitch + lay.cols);
     }
-    __device__ __forceinline__ char* Slot(const Group& g, uint32_t turn, int i) const {
+    __device__ __forceinline__ char* Slot(uint32_t turn, int i) const {
         if constexpr (V > 1) return slots + (turn * NV + i) * (kThreads * kPackBytes);
-        else return slots + turn * g.count * line_bytes;
+        else return slots + turn * (kThreads / Lay::L * kLineBytes);
     }
-    // The group's next row, zeros where there is none left.
-    __device__ __forceinline__ void Fetch(const Group& g, uint32_t turn, bool in) {
+    // The group's next row, zeros (V > 1) where there is none left.
+    __device__ __forceinline__ void Fetch(const Lay& lay, uint32_t turn, bool in) {
         if constexpr (V > 1) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (PackColumn<V>(g, i) >= cols) continue;
-                if (in) CopyAsync<kPackBytes>(static_cast<uint32_t>(__cvta_generic_to_shared(Slot(g, turn, i))), next + i * g.lanes * V);
-                else *reinterpret_cast<typename Word<kPackBytes>::type*>(Slot(g, turn, i)) = {};
-            }
+            lay.Each([&](int i, bool has) {
+                if (!has) return;
+                if (in) CopyAsync<kPackBytes>(static_cast<uint32_t>(__cvta_generic_to_shared(Slot(turn, i))), next + lay.Offset(i));
+                else *reinterpret_cast<typename Word<kPackBytes>::type*>(Slot(turn, i)) = {};
+            });
         } else if (in) {
-            const uintptr_t begin = reinterpret_cast<uintptr_t>(next), end = begin + static_cast<uintptr_t>(cols) * sizeof(T);
-            char* to = Slot(g, turn, 0) + 16U * g.lane;
-            for (uintptr_t line = (begin & ~static_cast<uintptr_t>(15)) + 16U * g.lane; line < end; line += 16U * g.lanes, to += 16U * g.lanes) {
-                if (line >= least && line + 16U <= most) {
-                    CopyAsync<16>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), reinterpret_cast<const void*>(line));
-                } else {
-                    for (uintptr_t e = line < begin ? begin : line; e < end && e < line + 16U; e += sizeof(T))
-                        *reinterpret_cast<T*>(to + (e - line)) = *reinterpret_cast<const T*>(e);
-                }
+            const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(next)) & 15U, lane = threadIdx.x % Lay::L;
+            const uint32_t bytes = (lay.end - lay.begin) * static_cast<uint32_t>(sizeof(T)) + shift, lines = (bytes + 15U) / 16U;
+            const uintptr_t first = reinterpret_cast<uintptr_t>(next) - shift;
+            char* to = Slot(turn, 0);
+            if (first >= least && first + lines * 16U <= most) {
+                const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to)) + 16U * lane;
+                const char* from = reinterpret_cast<const char*>(first) + 16U * lane;
+#pragma unroll
+                for (uint32_t k = 0; k < (kLineBytes / 16U + Lay::L - 1U) / Lay::L; ++k)
+                    if (k * Lay::L + lane < lines) CopyAsync<16>(at + k * Lay::L * 16U, from + k * Lay::L * 16U);
+            } else {
+                for (uint32_t e = shift + lane * static_cast<uint32_t>(sizeof(T)); e < bytes; e += Lay::L * static_cast<uint32_t>(sizeof(T)))
+                    *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(first + e);
             }
         }
         next += step;
     }
     // Before the first fetch: what lies beyond the row's end is zero in every slot and stays so (V > 1).
-    __device__ __forceinline__ void Clear(const Group& g) {
+    __device__ __forceinline__ void Clear(const Lay& lay) {
         if constexpr (V > 1) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (PackColumn<V>(g, i) >= cols)
-                    for (uint32_t turn = 0; turn < kDepth; ++turn) *reinterpret_cast<typename Word<kPackBytes>::type*>(Slot(g, turn, i)) = {};
+            lay.Each([&](int i, bool has) {
+                if (has) return;
+                for (uint32_t turn = 0; turn < kDepth; ++turn) *reinterpret_cast<typename Word<kPackBytes>::type*>(Slot(turn, i)) = {};
+            });
         }
     }
-    // This thread's elements of a row that has arrived; zeros beyond the row's end, and where there is no row.
-    __device__ __forceinline__ void Read(Held<NV * V>& out, const Group& g, uint32_t turn, bool in) {
+    // This thread's elements of a row that has arrived; zeros beyond the row's end, and where there is no row (what a line holds that nothing was
+    // copied to is read there and left aside).
+    __device__ __forceinline__ void Read(Held<V * NV>& out, const Lay& lay, uint32_t turn, bool in) {
         if constexpr (V > 1) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const Pack<T, V> p = LoadPack<T, V>(reinterpret_cast<const T*>(Slot(g, turn, i)));
+                const Pack<T, V> p = LoadPack<T, V>(reinterpret_cast<const T*>(Slot(turn, i)));
 #pragma unroll
                 for (int j = 0; j < V / 2; ++j) out.pair[i * (V / 2) + j] = Up(reinterpret_cast<const typename Two<T>::type*>(&p)[j]);
             }
         } else {
-            const T* line = reinterpret_cast<const T*>(Slot(g, turn, 0) + (reinterpret_cast<uintptr_t>(now) & 15U));
+            const T* line = reinterpret_cast<const T*>(Slot(turn, 0) + (now & 15U)) + threadIdx.x % Lay::L;
+            lay.Each([&](int i, bool has) { out.Set(i, has ? ToFloat(line[i * Lay::L]) : 0.0f); });
+            if (!in) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t c = PackColumn<V>(g, i);
-                out.Set(i, in && c < cols ? ToFloat(line[c]) : 0.0f);
+                for (int k = 0; k < Held<V * NV>::kPairs; ++k) out.pair[k] = Both(0.0f);
             }
-            now += step;
+            now += now_step;
         }
     }
 };
@@ -262,25 +293,13 @@ __device__ __forceinline__ Pack<T, V> PackOf(const Held<E>& v, int i) {
     }
     return p;
 }
-// `value` where the thread's elements are in the row, zero where they are not.
-template <int V, int NV>
-__device__ __forceinline__ void InRow(Held<NV * V>& out, const Group& g, uint32_t cols, float value) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const float v = PackColumn<V>(g, i) < cols ? value : 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) out.Set(i * V + j, v);
-    }
-}
 // A vector of columns that may begin anywhere; `none` for no vector, zero beyond the row's end.
-template <int V, int NV>
-__device__ __forceinline__ void LoadColumns(Held<NV * V>& out, const Group& g, uint32_t cols, const float* p, float none) {
+template <class Lay>
+__device__ __forceinline__ void LoadColumns(Held<Lay::E>& out, const Lay& lay, const float* p, float none) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t c = PackColumn<V>(g, i);
+    for (int i = 0; i < Lay::NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) out.Set(i * V + j, c < cols ? (p != nullptr ? p[c + j] : none) : 0.0f);
-    }
+        for (int j = 0; j < Lay::V; ++j) out.Set(i * Lay::V + j, lay.Has(i) ? (p != nullptr ? p[lay.base + lay.Offset(i) + j] : none) : 0.0f);
 }
 template <int E>
 __device__ __forceinline__ float SumOf(const Held<E>& v) {
@@ -289,16 +308,10 @@ __device__ __forceinline__ float SumOf(const Held<E>& v) {
     for (int k = 1; k < Held<E>::kPairs; ++k) s = Add2(s, v.pair[k]);
     return s.x + s.y;
 }
-// Everybody of the group sees what the group copied, or has read what it will overwrite.
-__device__ __forceinline__ void GroupBarrier(const Group& g) {
-    if (g.lanes <= 32U) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(1U + g.index), "r"(g.lanes) : "memory");
-}
-
 // ---- host side: how a row is cut
 constexpr uint32_t kMostLanes = 512, kElements = 16;
 struct Cut {
-    int nv;              // packs a thread: 1, 2, 4, 8 or 16
+    uint32_t nv;         // packs a thread
     uint32_t lanes, threads;
     bool stream;         // wider than a CTA holds
 };
@@ -316,11 +329,31 @@ inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v) {
         return c;
     }
     c.lanes = PowerOfTwo((packs - 1U) / most + 1U);
-    if (v == 1U && c.lanes < 4U) c.lanes = 4;  // (a line of 16 bytes and more a row: not too many rows a CTA)
+    if (v == 1U && c.lanes != 8U) c.lanes = c.lanes < 8U ? 8U : c.lanes < 32U ? 32U : c.lanes;  // stretches of 8 or 32 lanes
     while (c.lanes < 256U && c.lanes < packs && static_cast<uint64_t>(rows) * c.lanes < 148ULL * 512ULL) c.lanes <<= 1;
-    c.nv = static_cast<int>(PowerOfTwo((packs - 1U) / c.lanes + 1U));
+    c.nv = (packs - 1U) / c.lanes + 1U;
     if (c.lanes > c.threads) c.threads = c.lanes;
     return c;
+}
+// Single columns: the layout with the fewest turns that hold a stretch, and with turns to mask for all numbers of columns that come to it.
+template <class T>
+struct Tag {
+    using type = T;
+};
+template <class F>
+inline mgt_status_t SingleColumns(const Cut& cut, F run) {
+    if (cut.lanes < 32U) {
+        if (cut.nv <= 2U) return run(Tag<Layout<1, 2, 8, 2>>{});
+        if (cut.nv <= 4U) return run(Tag<Layout<1, 4, 8, 2>>{});
+        if (cut.nv <= 8U) return run(Tag<Layout<1, 8, 8, 4>>{});
+        return run(Tag<Layout<1, 16, 8, 8>>{});
+    }
+    if (cut.nv <= 2U) return run(Tag<Layout<1, 2, 32, 2>>{});
+    if (cut.nv <= 4U) return run(Tag<Layout<1, 4, 32, 2>>{});
+    if (cut.nv <= 6U) return run(Tag<Layout<1, 6, 32, 2>>{});
+    if (cut.nv <= 8U) return run(Tag<Layout<1, 8, 32, 2>>{});
+    if (cut.nv <= 12U) return run(Tag<Layout<1, 12, 32, 4>>{});
+    return run(Tag<Layout<1, 16, 32, 4>>{});
 }
 // Dynamic shared memory beyond 48 KB is an attribute of a kernel on a device: set on the first launch there.
 template <class Kernel>

@@ -16,14 +16,15 @@ constexpr uint32_t kColumnSlices = 37;  // widest rows: slices of the batch that
 inline __host__ __device__ uint32_t PartialPitch(uint32_t cols) { return (cols + 3U) / 4U * 4U; }
 
 // What a kernel is made of: packs of a thread, threads, rows on their way, CTAs an SM.
-template <class Tdy, class Tx, int V_, int NV_, int kThreads_>
+template <class Tdy, class Tx, class Lay_, int kThreads_>
 struct Form {
-    static constexpr int V = V_, NV = NV_, kThreads = kThreads_, E = V * NV;
+    using Lay = Lay_;
+    static constexpr int V = Lay::V, kThreads = kThreads_, E = Lay::E;
     static constexpr int kBytes = E * (sizeof(Tdy) + sizeof(Tx)) * kThreads;  // of a row of every group
     static constexpr int kDepth = V == 1 || kBytes > (32 << 10) ? 2 : kBytes >= (16 << 10) ? 3 : 6;
     static constexpr int kCtas = kThreads > 256 ? 1 : 2;
-    using RingDy = Ring<Tdy, V, NV, kThreads, kDepth>;
-    using RingX = Ring<Tx, V, NV, kThreads, kDepth>;
+    using RingDy = Ring<Tdy, Lay, kThreads, kDepth>;
+    using RingX = Ring<Tx, Lay, kThreads, kDepth>;
     static constexpr uint32_t kGammaBytes = E * kThreads * 4U;
 };
 
@@ -31,39 +32,38 @@ template <class Tdy, class Tx, class Tdx, class F>
 __global__ void __launch_bounds__(F::kThreads, F::kCtas)
 BackwardKernel(const Backward a) {
     extern __shared__ __align__(16) char memory[];  // gamma, the rings; at the end [groups][cols] sums, where there is more than one group
-    constexpr int V = F::V, NV = F::NV, E = F::E, D = F::kDepth, kThreads = F::kThreads, kPairs = Held<E>::kPairs;
+    using Lay = typename F::Lay;
+    constexpr int V = F::V, E = F::E, D = F::kDepth, kThreads = F::kThreads, kPairs = Held<E>::kPairs;
     __shared__ float buffer[2 * 2 * (kThreads / 32)];
     Group g = MakeGroup(a.lanes, buffer);
     const Share share = MakeShare(g, a.rows);
-    typename F::RingDy ring_dy(a.dy, a.dy_pitch, a.rows, a.cols, memory + F::kGammaBytes, g, share);
-    typename F::RingX ring_x(a.x, a.x_pitch, a.rows, a.cols, memory + F::kGammaBytes + F::RingDy::Bytes(a.cols, g.count), g, share);
+    const Lay lay(g, a.cols);
+    typename F::RingDy ring_dy(a.dy, a.dy_pitch, a.rows, memory + F::kGammaBytes, share, lay);
+    typename F::RingX ring_x(a.x, a.x_pitch, a.rows, memory + F::kGammaBytes + F::RingDy::kBytes, share, lay);
     const float per_col = 1.0f / static_cast<float>(a.cols);
-    Tdx* dx = static_cast<Tdx*>(a.dx) + share.first * a.dx_pitch + g.lane * V;
+    Tdx* dx = static_cast<Tdx*>(a.dx) + share.first * a.dx_pitch + lay.base;
     const uint64_t dx_step = share.stride * a.dx_pitch;
-    ring_dy.Clear(g);
-    ring_x.Clear(g);
+    ring_dy.Clear(lay);
+    ring_x.Clear(lay);
     dependent_begin();
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-        ring_dy.Fetch(g, d, d < share.mine);
-        ring_x.Fetch(g, d, d < share.mine);
+        ring_dy.Fetch(lay, d, d < share.mine);
+        ring_x.Fetch(lay, d, d < share.mine);
         CopiesEnd();
     }
     float next_mean, next_rstd;
-    const float* mean_at = a.mean + share.first;
-    const float* rstd_at = a.rstd + share.first;
     auto load_statistics = [&](uint32_t t) {  // (a row that is not there adds nothing to the sums)
-        next_mean = t < share.mine ? *mean_at : 0.0f;
-        next_rstd = t < share.mine ? *rstd_at : 0.0f;
-        mean_at += share.stride;
-        rstd_at += share.stride;
+        const uint32_t row = share.first + t * share.stride;
+        next_mean = t < share.mine ? a.mean[row] : 0.0f;
+        next_rstd = t < share.mine ? a.rstd[row] : 0.0f;
     };
     load_statistics(0);
-    float4* gamma_at = reinterpret_cast<float4*>(memory) + threadIdx.x;  // this thread's columns: in registers they would spill beside the sums
-    Held<E> gy, xhat, gamma, sums[kSums];
-    LoadColumns<V, NV>(gamma, g, a.cols, a.gamma, 1.0f);
+    float2* gamma_at = reinterpret_cast<float2*>(memory) + threadIdx.x;  // this thread's columns: in registers they would spill beside the sums
+    Held<E> gy, xhat, sums[kSums];
+    LoadColumns(xhat, lay, a.gamma, 1.0f);
 #pragma unroll
-    for (int k = 0; k < E; k += 4) gamma_at[k / 4 * kThreads] = make_float4(gamma.Get(k), gamma.Get(k + 1), gamma.Get(k + 2), gamma.Get(k + 3));
+    for (int k = 0; k < kPairs; ++k) gamma_at[k * kThreads] = xhat.pair[k];
 #pragma unroll
     for (uint32_t n = 0; n < kSums; ++n)
 #pragma unroll
@@ -74,30 +74,24 @@ BackwardKernel(const Backward a) {
         const float2 less = Both(-next_mean), rstd = Both(next_rstd);
         load_statistics(t + 1U);
         CopiesWait<D - 1>();
-        if (V == 1) GroupBarrier(g);
-        ring_dy.Read(gy, g, slot, in);
-        ring_x.Read(xhat, g, slot, in);
-#pragma unroll
-        for (int k = 0; k < E; k += 4) {
-            const float4 q = gamma_at[k / 4 * kThreads];
-            gamma.pair[k / 2] = make_float2(q.x, q.y);
-            gamma.pair[k / 2 + 1] = make_float2(q.z, q.w);
-        }
+        if (V == 1) __syncwarp();  // (what the other lanes copied is here, too)
+        ring_dy.Read(gy, lay, slot, in);
+        ring_x.Read(xhat, lay, slot, in);
         float2 s1 = Both(0.0f), s2 = Both(0.0f);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {  // (beyond the row's end dy is zero, and with it all that xhat enters)
             xhat.pair[k] = Mul2(Add2(xhat.pair[k], less), rstd);
             sums[0].pair[k] = Fma2(gy.pair[k], xhat.pair[k], sums[0].pair[k]);
             sums[1].pair[k] = Add2(gy.pair[k], sums[1].pair[k]);
-            gy.pair[k] = Mul2(gy.pair[k], gamma.pair[k]);
+            gy.pair[k] = Mul2(gy.pair[k], gamma_at[k * kThreads]);
             s1 = Add2(s1, gy.pair[k]);
             s2 = Fma2(gy.pair[k], xhat.pair[k], s2);
         }
         float s[2] = {s1.x + s1.y, s2.x + s2.y};
         Reduce(g, s);
-        if (V == 1) GroupBarrier(g);  // (everybody has what it read of the slot: the sums needed it)
-        ring_dy.Fetch(g, slot, t + D < share.mine);
-        ring_x.Fetch(g, slot, t + D < share.mine);
+        if (V == 1) __syncwarp();  // (everybody has what it read of the slot: the sums needed it)
+        ring_dy.Fetch(lay, slot, t + D < share.mine);
+        ring_x.Fetch(lay, slot, t + D < share.mine);
         CopiesEnd();
         slot = slot + 1U == D ? 0U : slot + 1U;
         if (in) {
@@ -107,9 +101,9 @@ BackwardKernel(const Backward a) {
                 gy.pair[k] = Mul2(rstd, Fma2(xhat.pair[k], c2, Add2(gy.pair[k], c1)));  // (rstd last: it is large where the differences are small)
                 sums[2].pair[k] = Add2(gy.pair[k], sums[2].pair[k]);  // (before it is rounded to dx's type; beyond the row's end nobody looks)
             }
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (PackColumn<V>(g, i) < a.cols) StorePack<Tdx, V>(dx + i * g.lanes * V, PackOf<Tdx, V>(gy, i));
+            lay.Each([&](int i, bool has) {
+                if (has) StorePack<Tdx, V>(dx + lay.Offset(i), PackOf<Tdx, V>(gy, i));
+            });
         }
         dx += dx_step;
     }
@@ -125,12 +119,10 @@ BackwardKernel(const Backward a) {
         float* to = gridDim.x > 1U ? partial + k * pitch : a.sums[k];
         float* mine = g.count > 1U ? lanes_sums + g.index * a.cols : to;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = PackColumn<V>(g, i);
+        for (int i = 0; i < Lay::NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (c < a.cols) mine[c + j] = sums[k].Get(i * V + j);
-        }
+                if (lay.Has(i)) mine[lay.base + lay.Offset(i) + j] = sums[k].Get(i * V + j);
         if (g.count > 1U) {
             __syncthreads();
             for (uint32_t c = threadIdx.x; c < a.cols; c += kThreads) {
@@ -249,7 +241,7 @@ mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint64_t want = (static_cast<uint64_t>(a.rows) + groups - 1U) / groups;
     const uint32_t most = kSms * F::kCtas, ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
-    const uint32_t rings = F::kGammaBytes + F::RingDy::Bytes(a.cols, groups) + F::RingX::Bytes(a.cols, groups);
+    const uint32_t rings = F::kGammaBytes + F::RingDy::kBytes + F::RingX::kBytes;
     const uint32_t sums = groups > 1U ? groups * a.cols * 4U : 0U, smem = rings > sums ? rings : sums;
     static std::atomic<uint64_t> allowed{0};
     if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, F>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
@@ -271,11 +263,16 @@ mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
         SumPartialRows(a, used, on, launches);
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
-    // (packs that the kernel has room for and the row does not have lie beyond its end)
-    constexpr int kMost = kElements / V, kFew = V == 1 ? 4 : V == 4 ? 2 : 1;
-    if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, V, kMost, 512>>(a, cut, on, launches);
-    if (cut.nv <= kFew) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, V, kFew, 256>>(a, cut, on, launches);
-    return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, V, kMost, 256>>(a, cut, on, launches);
+    // (packs that a kernel has room for and the row does not have lie beyond its end)
+    constexpr int kMost = kElements / V;
+    if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512>>(a, cut, on, launches);
+    if constexpr (V == 1) {
+        return SingleColumns(cut, [&](auto tag) { return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, typename decltype(tag)::type, 256>>(a, cut, on, launches); });
+    } else {
+        constexpr int kFew = V == 4 ? 2 : 1;
+        if (cut.nv <= kFew) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kFew, 32, 0>, 256>>(a, cut, on, launches);
+        return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, 0>, 256>>(a, cut, on, launches);
+    }
 }
 template <class Tdy, class Tx, class Tdx>
 mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {

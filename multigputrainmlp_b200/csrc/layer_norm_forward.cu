@@ -17,53 +17,62 @@ __device__ __forceinline__ Moments Finish(float first, const float (&sums)[2], f
     return {first + shift, shift, r * fmaf(-0.5f * v * r, r, 1.5f)};  // one Newton step: to an ulp, at a tenth of a root's and a division's price
 }
 
-template <class Tx, int V, int NV>
-constexpr int kDepth = V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : NV * V * sizeof(Tx) >= 64 ? 3 : NV * V * sizeof(Tx) >= 32 ? 5 : 8;
-constexpr uint32_t kCtasPerSm = 3;
+template <class Tx, class Lay>
+constexpr int kDepth = Lay::V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : Lay::E * sizeof(Tx) >= 64 ? 3 : Lay::E * sizeof(Tx) >= 32 ? 5 : 8;
+template <class Lay, int kThreads>
+constexpr uint32_t kCtas = kThreads > 256 ? 1 : Lay::V == 1 && Lay::E > 8 ? 2 : 3;  // an SM (single columns take more registers)
 
 // kTower: x is a layer's output before its normalisation, the normalised row is added to the fp32 residual stream, and what a ReLU leaves
 // goes to the stream and, as the next product's operand, to y.
-template <class Tx, class Ty, int V, int NV, int kThreads, bool kTower>
-__global__ void __launch_bounds__(kThreads, kThreads == 256 ? kCtasPerSm : 1)
+template <class Tx, class Ty, class Lay, int kThreads, bool kTower>
+__global__ void __launch_bounds__(kThreads, kCtas<Lay, kThreads>)
 ForwardKernel(const Forward a) {
     extern __shared__ __align__(16) char memory[];
     __shared__ float buffer[2 * 2 * (kThreads / 32)];
-    constexpr int D = kDepth<Tx, V, NV>, kPairs = Held<NV * V>::kPairs;
+    constexpr int V = Lay::V, E = Lay::E, D = kDepth<Tx, Lay>, kPairs = Held<E>::kPairs;
     Group g = MakeGroup(a.lanes, buffer);
     const Share share = MakeShare(g, a.rows);
-    Ring<Tx, V, NV, kThreads, D> ring(a.x, a.x_pitch, a.rows, a.cols, memory, g, share);
+    const Lay lay(g, a.cols);
+    Ring<Tx, Lay, kThreads, D> ring(a.x, a.x_pitch, a.rows, memory, share, lay);
     const float per_col = 1.0f / static_cast<float>(a.cols);
-    Ty* y = static_cast<Ty*>(a.y) + share.first * a.y_pitch + g.lane * V;
-    float* state = kTower ? a.state + share.first * a.x_pitch + g.lane * V : nullptr;
+    Ty* y = static_cast<Ty*>(a.y) + share.first * a.y_pitch + lay.base;
+    float* state = kTower ? a.state + share.first * a.x_pitch + lay.base : nullptr;
     const uint64_t y_step = share.stride * a.y_pitch, state_step = share.stride * a.x_pitch;
-    ring.Clear(g);
+    ring.Clear(lay);
     dependent_begin();
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-        ring.Fetch(g, d, d < share.mine);
+        ring.Fetch(lay, d, d < share.mine);
         CopiesEnd();
     }
-    Held<NV * V> gamma, beta, m, v;
-    LoadColumns<V, NV>(gamma, g, a.cols, a.gamma, 1.0f);
-    LoadColumns<V, NV>(beta, g, a.cols, a.beta, 0.0f);
+    Held<E> gamma, beta, v;
+    LoadColumns(gamma, lay, a.gamma, 1.0f);
+    LoadColumns(beta, lay, a.beta, 0.0f);
     uint32_t slot = 0, row = share.first;
     for (uint32_t t = 0; t < share.turns; ++t) {
         const bool in = t < share.mine;
         CopiesWait<D - 1>();
-        if (V == 1) GroupBarrier(g);
-        ring.Read(v, g, slot, in);
+        if (V == 1) __syncwarp();  // (what the other lanes copied is here, too)
+        ring.Read(v, lay, slot, in);
         float sum[1] = {SumOf(v)};
         Reduce(g, sum);
-        if (V == 1) GroupBarrier(g);  // (everybody has what it read of the slot: the sum needed it)
-        ring.Fetch(g, slot, t + D < share.mine);
+        if (V == 1) __syncwarp();  // (everybody has what it read of the slot: the sum needed it)
+        ring.Fetch(lay, slot, t + D < share.mine);
         CopiesEnd();
         slot = slot + 1U == D ? 0U : slot + 1U;
         const float first = sum[0] * per_col;
-        InRow<V, NV>(m, g, a.cols, -first);
+        if constexpr (V > 1) {
+            lay.Each([&](int i, bool has) {
+                const float2 m = Both(has ? -first : 0.0f);
+#pragma unroll
+                for (int k = 0; k < V / 2; ++k) v.pair[i * (V / 2) + k] = Add2(v.pair[i * (V / 2) + k], m);
+            });
+        } else {
+            lay.Each([&](int i, bool has) { v.Set(i, has ? v.Get(i) - first : 0.0f); });
+        }
         float2 s1 = Both(0.0f), s2 = Both(0.0f);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {
-            v.pair[k] = Add2(v.pair[k], m.pair[k]);
             s1 = Add2(s1, v.pair[k]);
             s2 = Fma2(v.pair[k], v.pair[k], s2);
         }
@@ -78,10 +87,9 @@ ForwardKernel(const Forward a) {
             const float2 rstd = Both(mo.rstd), off = Both(-mo.shift * mo.rstd);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) v.pair[k] = Fma2(Fma2(v.pair[k], rstd, off), gamma.pair[k], beta.pair[k]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (PackColumn<V>(g, i) >= a.cols) continue;
-                const uint32_t at = i * g.lanes * V;
+            lay.Each([&](int i, bool has) {
+                if (!has) return;
+                const uint32_t at = lay.Offset(i);
                 if (kTower) {
                     const Pack<float, V> old = a.add ? LoadPack<float, V>(state + at) : Pack<float, V>{};
 #pragma unroll
@@ -89,7 +97,7 @@ ForwardKernel(const Forward a) {
                     StorePack<float, V>(state + at, PackOf<float, V>(v, i));
                 }
                 StorePack<Ty, V>(y + at, PackOf<Ty, V>(v, i));
-            }
+            });
         }
         y += y_step;
         if (kTower) state += state_step;
@@ -149,38 +157,45 @@ StreamForwardKernel(const Forward a) {
 
 constexpr int kMostShared = 110 << 10;
 
-template <class Tx, class Ty, int V, int NV, int kThreads, bool kTower>
+template <class Tx, class Ty, class Lay, int kThreads, bool kTower>
 mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
     const uint32_t rows = cut.threads / cut.lanes;
     const uint64_t want = (static_cast<uint64_t>(a.rows) + rows - 1U) / rows;
     a.lanes = cut.lanes;
     static std::atomic<uint64_t> allowed{0};
-    const uint32_t smem = Ring<Tx, V, NV, kThreads, kDepth<Tx, V, NV>>::Bytes(a.cols, rows);
-    if (!AllowShared(ForwardKernel<Tx, Ty, V, NV, kThreads, kTower>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
-    const uint32_t most = 148U * (cut.threads == 256U ? kCtasPerSm : 1U);
-    Launch(ForwardKernel<Tx, Ty, V, NV, kThreads, kTower>, static_cast<uint32_t>(want < most ? want : most), cut.threads, smem, on, a);
+    const uint32_t smem = Ring<Tx, Lay, kThreads, kDepth<Tx, Lay>>::kBytes;
+    if (!AllowShared(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
+    const uint32_t most = 148U * kCtas<Lay, kThreads>;
+    Launch(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, static_cast<uint32_t>(want < most ? want : most), cut.threads, smem, on, a);
     return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
 }
-template <class Tx, class Ty, int V>
+// (packs that a kernel has room for and the row does not have lie beyond its end)
+template <class Tx, class Ty, int V, bool kTower>
 mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
     const Cut cut = CutRow(a.rows, a.cols, V);
-    if (cut.stream) {
+    constexpr int kMost = kElements / V;
+    if (cut.stream || (kTower && cut.threads > 256U)) {
+        if constexpr (kTower) return MGT_INVALID_CONFIG;  // (no tower is that wide)
         Launch(StreamForwardKernel<Tx, Ty, V>, a.rows < 296U ? a.rows : 296U, 1024, 0, on, a);
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
-    constexpr int kMost = kElements / V, kFew = V == 1 ? 4 : 2;  // packs a thread that there are kernels for, besides one
-    if (cut.threads > 256U) return Run<Tx, Ty, V, kMost, 512, false>(a, cut, on);
-    if (cut.nv == 1) return Run<Tx, Ty, V, 1, 256, false>(a, cut, on);
-    if (cut.nv <= kFew) return Run<Tx, Ty, V, kFew, 256, false>(a, cut, on);
-    return Run<Tx, Ty, V, kMost, 256, false>(a, cut, on);
+    if constexpr (!kTower)
+        if (cut.threads > 256U) return Run<Tx, Ty, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512, false>(a, cut, on);
+    if constexpr (V == 1) {
+        return SingleColumns(cut, [&](auto tag) { return Run<Tx, Ty, typename decltype(tag)::type, 256, kTower>(a, cut, on); });
+    } else {
+        if (cut.nv == 1) return Run<Tx, Ty, Layout<V, 1, 32, 0>, 256, kTower>(a, cut, on);
+        if (cut.nv == 2) return Run<Tx, Ty, Layout<V, 2, 32, 0>, 256, kTower>(a, cut, on);
+        return Run<Tx, Ty, Layout<V, kMost, 32, 0>, 256, kTower>(a, cut, on);
+    }
 }
 template <class Tx, class Ty>
 mgt_status_t RunTyped(const Forward& a, int32_t x_type, int32_t y_type, LaunchOn on) {
     auto whole = [&](int v) { return a.cols % v == 0 && RowsAligned(a.x, a.x_pitch, a.rows, x_type, v) && RowsAligned(a.y, a.y_pitch, a.rows, y_type, v); };
     if constexpr (sizeof(Tx) == 2 && sizeof(Ty) == 2)
-        if (whole(8)) return RunByWidth<Tx, Ty, 8>(a, on);
-    if (whole(4)) return RunByWidth<Tx, Ty, 4>(a, on);
-    return RunByWidth<Tx, Ty, 1>(a, on);
+        if (whole(8)) return RunByWidth<Tx, Ty, 8, false>(a, on);
+    if (whole(4)) return RunByWidth<Tx, Ty, 4, false>(a, on);
+    return RunByWidth<Tx, Ty, 1, false>(a, on);
 }
 
 }  // namespace
@@ -197,17 +212,9 @@ mgt_status_t LaunchForward(Forward a, int32_t x_type, int32_t y_type, LaunchOn o
 }
 
 mgt_status_t LaunchTowerForward(Forward a, bool bf16, LaunchOn on) {
-    const uint32_t v = a.cols % 4U == 0 && a.x_pitch % 4U == 0 && a.y_pitch % 4U == 0 ? 4U : 1U;
-    const Cut cut = CutRow(a.rows, a.cols, v);
-    if (cut.threads > 256U || cut.stream) return MGT_INVALID_CONFIG;  // (no tower is that wide)
-    auto run = [&](auto type) {
-        using T = decltype(type);
-        if (v == 1U) return cut.nv <= 4 ? Run<float, T, 1, 4, 256, true>(a, cut, on) : Run<float, T, 1, 16, 256, true>(a, cut, on);
-        if (cut.nv == 1) return Run<float, T, 4, 1, 256, true>(a, cut, on);
-        if (cut.nv == 2) return Run<float, T, 4, 2, 256, true>(a, cut, on);
-        return Run<float, T, 4, 4, 256, true>(a, cut, on);
-    };
-    return bf16 ? run(__nv_bfloat16{}) : run(__half{});
+    const bool whole = a.cols % 4U == 0 && a.x_pitch % 4U == 0 && a.y_pitch % 4U == 0;
+    if (bf16) return whole ? RunByWidth<float, __nv_bfloat16, 4, true>(a, on) : RunByWidth<float, __nv_bfloat16, 1, true>(a, on);
+    return whole ? RunByWidth<float, __half, 4, true>(a, on) : RunByWidth<float, __half, 1, true>(a, on);
 }
 
 }  // namespace ln
