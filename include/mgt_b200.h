@@ -177,6 +177,16 @@ mgt_status_t mgt_engine_set_batch_norm_state(mgt_engine_t* engine, float* device
                                              uint32_t world_size, float* device_exchange_buffer,
                                              mgt_stats_exchange_fn exchange, void* user);
 
+/* Layer normalisation in the places of the batch normalisation above (the hidden layer's pre-activation before its ReLU, every
+ * residual block's fc2 output before the skip add), with the same scale/shift vectors behind the parameters (mgt_bn_param_count
+ * floats) and the same one range more for gradient_ready: every sample is normalised by itself, so nothing is exchanged between
+ * ranks and there are no running statistics - and nothing that could be folded into the weights. Off by default. Needs
+ * use_half_linear = 1 and excludes batch_norm (the launch returns MGT_INVALID_CONFIG otherwise); goes with either operand format and loss.
+ * The workspace is larger: mgt_mlp_loss_grad_workspace_floats_with_layer_norm. eps > 0 and finite. */
+mgt_status_t mgt_engine_set_layer_norm(mgt_engine_t* engine, int32_t enabled, float eps);
+uint64_t mgt_mlp_loss_grad_workspace_floats_with_layer_norm(const mgt_mlp_shape_t* shape, uint32_t sample_count,
+                                                            uint32_t input_grad_partial_chunks, int32_t use_half_input_grad);
+
 /* Early-range hook (optional; no counterpart in the reference). The embedding table and the input bias are 86 % of the
  * p888 parameters and the reference announces them last. This library computes their gradient BEFORE the weight-gradient
  * GEMMs of the residual blocks and of the hidden layer, and calls `hook` (same signature and rules as gradient_ready;

@@ -51,6 +51,9 @@ def _declare(lib: C.CDLL) -> None:
     lib.mgt_validate_adamw_config.argtypes = [vp]
     lib.mgt_launch_adamw.argtypes = [vp, vp, vp, vp, vp, vp]
     lib.mgt_launch_adamw_with_half_mirror.argtypes = [vp, vp, vp, vp, vp, vp, vp]
+    lib.mgt_engine_set_layer_norm.argtypes = [vp, i32, f32]
+    lib.mgt_mlp_loss_grad_workspace_floats_with_layer_norm.restype = u64
+    lib.mgt_mlp_loss_grad_workspace_floats_with_layer_norm.argtypes = [vp, u32, u32, i32]
     lib.mgt_launch_adamw_with_clip.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp]
     lib.mgt_validate_layer_norm_config.argtypes = [vp]
     lib.mgt_launch_layer_norm.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp]

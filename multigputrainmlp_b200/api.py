@@ -204,9 +204,12 @@ class _TrainOptions(C.Structure):
 
 
 def mlp_loss_grad_workspace_floats(shape, sample_count, input_grad_partial_chunks=1, use_half_input_grad=True,
-                                   use_half_linear=True, batch_norm=False) -> int:
+                                   use_half_linear=True, batch_norm=False, layer_norm=False) -> int:
     s = shape.c()
     lib = _lib.load()
+    if layer_norm:  # (neither beside batch normalisation nor all in fp32)
+        return 0 if batch_norm or not use_half_linear else lib.mgt_mlp_loss_grad_workspace_floats_with_layer_norm(
+            C.byref(s), sample_count, input_grad_partial_chunks, int(use_half_input_grad))
     if not batch_norm:
         return int(lib.mgt_mlp_loss_grad_workspace_floats(C.byref(s), sample_count, input_grad_partial_chunks,
                                                           int(use_half_input_grad), int(use_half_linear)))
@@ -299,6 +302,10 @@ class Engine:
         self._lib.mgt_engine_set_batch_norm_state.argtypes = [C.c_void_p, C.c_void_p, C.c_float, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]
         return int(self._lib.mgt_engine_set_batch_norm_state(self.handle, _ptr(running_stats), momentum, world_size, buf,
                                                              C.cast(cb, C.c_void_p) if cb is not None else None, None))
+
+    def set_layer_norm(self, enabled: bool = True, eps: float = 1e-5) -> int:
+        """mgt_engine_set_layer_norm: layer normalisation where batch normalisation would be, every sample by itself."""
+        return self._lib.mgt_engine_set_layer_norm(self.handle, int(enabled), eps)
 
     def set_early_range_hook(self, fn=None) -> int:
         """mgt_engine_set_early_range_hook: fn(user, ready_id, offset, count, stream) -> status, or None to remove it."""

@@ -176,7 +176,7 @@ bool WriteWeights(const std::string& dir, const TrainPlan& plan, const std::vect
     man << "{\n  \"format\": \"stream1_weights\",\n  \"version\": 1,\n  \"state_len\": " << o.state_len << ",\n  \"num_classes\": " << o.state_value_count
         << ",\n  \"logical_num_classes\": " << o.state_value_count << ",\n  \"hd1\": " << E1 << ",\n  \"hd2\": " << E2 << ",\n  \"original_hd1\": " << o.hd1
         << ",\n  \"original_hd2\": " << o.hd2 << ",\n  \"hidden_alignment\": 8,\n  \"nrd\": " << o.nrd << ",\n  \"output_dim\": " << OUT
-        << ",\n  \"dtype\": \"fp16\",\n  \"normalization\": \"none\",\n  \"layout\": \"row-major input activations times weight_hxk\",\n"
+        << ",\n  \"dtype\": \"fp16\",\n  \"normalization\": \"" << (plan.options.layer_norm ? "layer_norm" : "none") << "\",\n  \"layout\": \"row-major input activations times weight_hxk\",\n"
         << "  \"flat_debug_weights\": \"weights.f32.bin\"\n}\n";
     return static_cast<bool>(man);
 }

@@ -13,6 +13,7 @@
 //   * activations are kept once (fp16 tape + one in-place fp32 residual stream).
 #include "../../include/mgt_b200.h"
 #include "batch_norm.cuh"
+#include "layer_norm.hpp"
 #include "embedding_gather.cuh"
 #include "fp32_path.cuh"
 #include "fp32_tower.cuh"
@@ -83,6 +84,8 @@ struct Workspace {
     uint32_t p_dz1_rows;
     uint64_t off_lists;
     uint64_t off_bn_z, bn_z_stride, off_bn_save, off_bn_partial, off_bn_bias, off_bn_stats;
+    // layer normalisation (likewise): the same tape of z, mean and rstd of every sample and layer, partial sums of the backward pass
+    uint64_t off_ln_save, off_ln_partial;
     uint64_t total_bytes;
 };
 
@@ -159,10 +162,12 @@ inline uint32_t MostSplits(uint32_t M, uint32_t N, uint32_t groups, uint32_t sm_
     return tiles >= sm_count ? 1U : (uint32_t)(sm_count / tiles);
 }
 
+enum class Norm { kNone, kBatch, kLayer };
+
 // No term may fall with a larger batch: a caller sizes its scratch for the largest batch and runs smaller ones in it. So what a
 // form of the embedding layer needs is planned whichever form this batch takes (288 bytes a sample of 72 positions). half_ig: the
 // table gradient is the 16-bit one (the fp32 one keeps its lists behind this workspace).
-Workspace PlanWorkspace(const mgt_mlp_shape_t& s, uint32_t B, uint32_t sm_count, bool half_ig, bool batch_norm = false) {
+Workspace PlanWorkspace(const mgt_mlp_shape_t& s, uint32_t B, uint32_t sm_count, bool half_ig, Norm norm) {
     Workspace w{};
     w.B = B; w.H1 = s.hd1; w.H2 = s.hd2; w.R = s.residual_blocks; w.OUT = s.output_dim;
     w.IN = s.state_len * s.state_value_pad;
@@ -221,9 +226,15 @@ Workspace PlanWorkspace(const mgt_mlp_shape_t& s, uint32_t B, uint32_t sm_count,
     w.off_wint = take(wint_halfs * 2 + 1024ULL * (2 * w.R + 4));
     w.off_dy = take((uint64_t)B * s.output_dim * 4);
     w.off_dyh = take((uint64_t)B * w.p_wout * 2);
-    if (batch_norm) {
+    if (norm != Norm::kNone) {
         w.bn_z_stride = RoundUp((uint64_t)B * w.p_f32 * 4, 1024);
         w.off_bn_z = take(w.bn_z_stride * (w.R + 1));
+    }
+    if (norm == Norm::kLayer) {
+        w.off_ln_save = take((uint64_t)(w.R + 1) * 2 * B * 4);
+        w.off_ln_partial = take(ln::BackwardFloats(B, s.hd2) * 4);
+    }
+    if (norm == Norm::kBatch) {
         w.off_bn_save = take((uint64_t)(w.R + 1) * 2 * s.hd2 * 4);
         w.off_bn_partial = take((uint64_t)bn::kMaxBlocks * 2 * s.hd2 * 4);
         w.off_bn_bias = take((uint64_t)(w.R + 1) * bn::kMaxBlocks * s.hd2 * 4);
@@ -367,6 +378,8 @@ struct mgt_engine {
     float* bn_exchange_buffer = nullptr;
     mgt_stats_exchange_fn bn_exchange = nullptr;
     void* bn_exchange_user = nullptr;
+    bool layer_norm = false;  // mgt_engine_set_layer_norm
+    float ln_eps = 1.0e-5f;
     bool bf16_now = false;  // operand format of the launch being enqueued (set by mgt_launch_mlp_loss_grad, off otherwise)
 
     // fp16 3-D tensor map (a stack of `layers` equal matrices `layer_stride_bytes` apart), 128-byte swizzle, box depth 1
@@ -1607,7 +1620,7 @@ mgt_status_t LaunchFp32Path(mgt_engine* e, const mgt_mlp_shape_t& s, const float
 // 4 096 samples of hd1 1024 210 -> 200 us, 5 003 of hd1 333 172 -> 157, 1 024 of hd1 256 103 -> 82; 3 001 samples of hd1 2560 make no
 // difference, and with kernels that fill the chip the next one's CTAs are in the way: 9 001 samples of hd1 1000 445 -> 491, 8 192 of
 // hd1 2560 in fp32 4 701 -> 5 230. The many passes of batch normalisation stream and gain at any size (53 248 of hd1 2560 5 884 -> 5 510).
-bool OverlapLaunches(const mgt_mlp_shape_t& s, uint32_t B, bool batch_norm) { return batch_norm || (uint64_t)B * s.hd1 <= 6000000ULL; }
+bool OverlapLaunches(const mgt_mlp_shape_t& s, uint32_t B, bool normed) { return normed || (uint64_t)B * s.hd1 <= 6000000ULL; }
 // All in fp32 the kernels have their operands through L1, and lose some of it to the shared memory of the next one, as soon as a
 // product has more than one or two tiles for an SM. Counted in tiles of 32 x 32, of the products by hd1 (the input gradient) and of those
 // by hd2 (the blocks): us a step without and with, by samples / hd1 / hd2 / blocks. Few tiles: 250 / 512 / 64 / 4 176 -> 153; 128 / 1000 /
@@ -1720,21 +1733,25 @@ static uint64_t Fp32TableFloats(const mgt_mlp_shape_t& s, uint32_t B) {
 }
 
 static uint64_t WorkspaceFloats(const mgt_mlp_shape_t* shape, uint32_t sample_count, uint32_t chunks, int32_t use_half_input_grad, int32_t use_half_linear,
-                                bool batch_norm) {
+                                Norm norm) {
     if (!ValidShape(shape) || sample_count == 0 || chunks == 0) return 0;
-    if (!use_half_linear) return batch_norm ? 0 : Fp32WorkspaceFloats(*shape, sample_count, CurrentDeviceSmCount());
-    const Workspace w = PlanWorkspace(*shape, sample_count, CurrentDeviceSmCount(), use_half_input_grad != 0, batch_norm);
+    if (!use_half_linear) return norm != Norm::kNone ? 0 : Fp32WorkspaceFloats(*shape, sample_count, CurrentDeviceSmCount());
+    const Workspace w = PlanWorkspace(*shape, sample_count, CurrentDeviceSmCount(), use_half_input_grad != 0, norm);
     return (w.total_bytes + 3) / 4 + (use_half_input_grad ? 0 : Fp32TableFloats(*shape, sample_count));
 }
 
 uint64_t mgt_mlp_loss_grad_workspace_floats(const mgt_mlp_shape_t* shape, uint32_t sample_count, uint32_t chunks,
                                             int32_t use_half_input_grad, int32_t use_half_linear) {
-    return WorkspaceFloats(shape, sample_count, chunks, use_half_input_grad, use_half_linear, false);
+    return WorkspaceFloats(shape, sample_count, chunks, use_half_input_grad, use_half_linear, Norm::kNone);
 }
 
 uint64_t mgt_mlp_loss_grad_workspace_floats_with_options(const mgt_mlp_shape_t* shape, uint32_t sample_count, uint32_t chunks, int32_t use_half_input_grad,
                                                          int32_t use_half_linear, const mgt_train_options_t* options) {
-    return WorkspaceFloats(shape, sample_count, chunks, use_half_input_grad, use_half_linear, options != nullptr && options->batch_norm != 0);
+    return WorkspaceFloats(shape, sample_count, chunks, use_half_input_grad, use_half_linear, options != nullptr && options->batch_norm != 0 ? Norm::kBatch : Norm::kNone);
+}
+
+uint64_t mgt_mlp_loss_grad_workspace_floats_with_layer_norm(const mgt_mlp_shape_t* shape, uint32_t sample_count, uint32_t chunks, int32_t use_half_input_grad) {
+    return WorkspaceFloats(shape, sample_count, chunks, use_half_input_grad, 1, Norm::kLayer);
 }
 
 uint64_t mgt_bn_param_count(const mgt_mlp_shape_t* shape) { return ValidShape(shape) ? 2ULL * (shape->residual_blocks + 1ULL) * shape->hd2 : 0; }
@@ -1763,8 +1780,9 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
         return MGT_INVALID_CONFIG;
     }
     const mgt_mlp_shape_t s = *shape;
-    const bool bnorm = e->options.batch_norm != 0;
-    const bool options_set = e->options.operand_format != MGT_OPERAND_FP16 || e->options.loss_kind != MGT_LOSS_MSE || bnorm;
+    const bool bnorm = e->options.batch_norm != 0, lnorm = e->layer_norm, normed = bnorm || lnorm;
+    if (bnorm && lnorm) return MGT_INVALID_CONFIG;
+    const bool options_set = e->options.operand_format != MGT_OPERAND_FP16 || e->options.loss_kind != MGT_LOSS_MSE || normed;
     if (options_set && !half_lin) return MGT_INVALID_CONFIG;  // the options belong to the tensor-core data flow
     if (e->options.loss_kind == MGT_LOSS_CROSS_ENTROPY && s.output_dim < 2U) return MGT_INVALID_CONFIG;
     struct FormatScope {  // the operand format applies to the kernels enqueued by this call only
@@ -1783,10 +1801,10 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
         return LaunchFp32Path(e, s, w, reinterpret_cast<const uint8_t*>(states), labels, B, loss, grad, workspace, half_ig != 0, ready != nullptr || profile != nullptr, profile, tell,
                               {static_cast<cudaStream_t>(stream_v), OverlapFp32Launches(s, B)});
     }
-    Workspace ws = PlanWorkspace(s, B, PlanSmCount(e->sm_count), half_ig != 0, bnorm);
+    Workspace ws = PlanWorkspace(s, B, PlanSmCount(e->sm_count), half_ig != 0, bnorm ? Norm::kBatch : lnorm ? Norm::kLayer : Norm::kNone);
     if (e->embedding_form != mgt_engine::kBySize) ws.gather_fwd = ws.gather_grad = e->embedding_form == mgt_engine::kGather;
     if (workspace_floats < (ws.total_bytes + 3) / 4 + (half_ig ? 0 : Fp32TableFloats(s, B))) return MGT_CAPACITY_EXCEEDED;
-    const LaunchOn st(static_cast<cudaStream_t>(stream_v), OverlapLaunches(s, B, bnorm));
+    const LaunchOn st(static_cast<cudaStream_t>(stream_v), OverlapLaunches(s, B, normed));
     uint8_t* base = reinterpret_cast<uint8_t*>(RoundUp(reinterpret_cast<uintptr_t>(workspace), 1024));
     float* dz1_f32 = reinterpret_cast<float*>(RoundUp(reinterpret_cast<uintptr_t>(workspace + (ws.total_bytes + 3) / 4), 256));  // behind the tensor-core workspace
     const uint32_t p_dz1_f32 = (uint32_t)RoundUp(s.hd1, 4);
@@ -1869,6 +1887,28 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     };
 
+    // ---- layer normalisation (opt-in): the same places and parameters, statistics of every sample by itself
+    auto ln_mean = [&](uint32_t layer) { return reinterpret_cast<float*>(base + ws.off_ln_save) + 2ULL * layer * B; };
+    // z_tape(layer) -> x_f32 / x_h(layer): x = relu(ln(z)) for the hidden layer, relu(x + ln(z)) for a block
+    auto ln_forward = [&](uint32_t layer) -> mgt_status_t {
+        const float* gamma = w + bn_base + 2ULL * layer * H2;
+        ++e->launches;
+        return ln::LaunchTowerForward({z_tape(layer), x_h(layer), gamma, gamma + H2, ln_mean(layer), ln_mean(layer) + B, x_f32, ws.p_f32, ws.p_act, B, H2, e->ln_eps, 0, layer != 0U},
+                                      e->bf16_now, st);
+    };
+    // dzf (gradient w.r.t. the sum entering the ReLU above the layer) -> dz_tape(layer) = gradient w.r.t. z, plus the
+    // gradients of gamma, beta and of the bias inside z
+    auto ln_backward = [&](uint32_t layer) -> mgt_status_t {
+        float* dgamma = grad + bn_base + 2ULL * layer * H2;
+        float* dbias = grad + (layer == 0U ? HiddenBias(s) : Fc2B(s, layer - 1U));
+        uint32_t launches = 0;
+        const mgt_status_t r = ln::LaunchBackward({dzf, z_tape(layer), dz_tape(layer), w + bn_base + 2ULL * layer * H2, ln_mean(layer), ln_mean(layer) + B, {dgamma, dgamma + H2, dbias},
+                                                   reinterpret_cast<float*>(base + ws.off_ln_partial), ws.p_f32, ws.p_f32, ws.p_dz, B, H2, 0},
+                                                  MGT_F32, MGT_F32, e->bf16_now ? MGT_BF16 : MGT_F16, st, &launches);
+        e->launches += launches;
+        return r;
+    };
+
     // ---- fp16 weights: the caller's mirror as it lies when TMA can address it, else a padded copy
     HalfWeights hw{};
     const __half* w_half = reinterpret_cast<const __half*>(w_half_u16);
@@ -1937,6 +1977,10 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
             MGT_TRY(bn_fused ? GemmForwardRows<Epi::kBiasF32Moments>(e, st, a1_h, ws.p_bt, hw.wh, hw.p2, B, H2, H1, epi)
                              : GemmForwardRows<Epi::kBiasF32>(e, st, a1_h, ws.p_bt, hw.wh, hw.p2, B, H2, H1, epi));
             MGT_TRY(bn_forward(0));
+        } else if (lnorm) {
+            epi.out_f32 = z_tape(0);
+            MGT_TRY(GemmForwardRows<Epi::kBiasF32>(e, st, a1_h, ws.p_bt, hw.wh, hw.p2, B, H2, H1, epi));
+            MGT_TRY(ln_forward(0));
         } else {
             MGT_TRY(GemmForwardRows<Epi::kBiasReluF32F16>(e, st, a1_h, ws.p_bt, hw.wh, hw.p2, B, H2, H1, epi));
         }
@@ -1944,7 +1988,7 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
     if (!timer.Mark(profile ? &profile->hidden_forward_ms : nullptr)) return MGT_CUDA_FAILURE;
 
     // ---- residual blocks forward (mlp_backward.cu:1294-1323)
-    const bool chain = ChainEligible(e, s) && !bnorm;  // batch statistics need the whole batch between two layers: one kernel per layer
+    const bool chain = ChainEligible(e, s) && !normed;  // batch statistics need the whole batch between two layers: one kernel per layer (and so with layer norm)
     const uint64_t w_layer_stride = R > 0 ? (uint64_t)(reinterpret_cast<const uint8_t*>(hw.w2[0]) - reinterpret_cast<const uint8_t*>(hw.w1[0])) : 16;
     ChainArgs ca{};
     ca.samples = B; ca.H = H2; ca.R = R; ca.tiles = (B + 127U) / 128U;
@@ -1975,6 +2019,12 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
             MGT_TRY(bn_forward(k + 1U));
             continue;
         }
+        if (lnorm) {
+            e2.out_f32 = z_tape(k + 1U);
+            MGT_TRY(GemmForward<Epi::kBiasF32>(e, st, r1_h(k), ws.p_act, hw.w2[k], hw.p2, B, H2, H2, e2));
+            MGT_TRY(ln_forward(k + 1U));
+            continue;
+        }
         MGT_TRY(GemmForward<Epi::kBiasResReluF32F16>(e, st, r1_h(k), ws.p_act, hw.w2[k], hw.p2, B, H2, H2, e2));
     }
     if (!timer.Mark(profile ? &profile->residual_forward_ms : nullptr)) return MGT_CUDA_FAILURE;
@@ -1982,7 +2032,7 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
     // ---- output head, loss and the gradient entering the last block (mlp_backward.cu:1327-1364)
     __half* dz_cur = dz_tape(R);   // fp16 copy of the gradient w.r.t. the pre-activation the head feeds
     // the head also yields the fp32 column sums of dz: the bias gradient of the layer below it, unless that is normalised
-    float* head_bias_dst = bnorm ? nullptr : grad + (R > 0 ? Fc2B(s, R - 1) : HiddenBias(s));
+    float* head_bias_dst = normed ? nullptr : grad + (R > 0 ? Fc2B(s, R - 1) : HiddenBias(s));
     if (OUT == 1U) {
         Launch(HeadOut1Kernel, kHeadBlocks, kHeadThreads, 0, st, w + OutputWeight(s), w + OutputBias(s), labels, x_f32, ws.p_f32, B, H2, dzf, dz_cur, ws.p_dz, head_partial, e->bf16_now);
         sums.Head(head_partial, kHeadBlocks, H2, grad + OutputWeight(s), loss, head_bias_dst);
@@ -2017,6 +2067,7 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
     }
     for (uint32_t rb = R; rb > 0 && !chain; --rb) {
         const uint32_t k = rb - 1U;
+        if (lnorm) MGT_TRY(ln_backward(k + 1U));
         if (bnorm) MGT_TRY(bn_backward(k + 1U));  // dz_tape(k + 1) = gradient w.r.t. the fc2 output; dzf goes down the skip path as it is
         GemmArgs d2{};  // dz1 = (dz2 * W2^T) * [r1 > 0]
         d2.mask = r1_h(k); d2.ld_mask = ws.p_act; d2.out_f16 = dz1_tape(k); d2.ld_f16 = ws.p_dz;
@@ -2035,6 +2086,7 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
 
     // ---- hidden layer backward, dX part (mlp_backward.cu:1417-1438): dz_tape(0) = dcur * [x0 > 0]
     dz_cur = dz_tape(0);
+    if (lnorm) MGT_TRY(ln_backward(0));
     if (bnorm) {
         MGT_TRY(bn_backward(0));
         // the gradients of the biases in front of the normalisations, of all layers
@@ -2124,8 +2176,8 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
         MGT_TRY(sums.Pass());
         MGT_TRY(GemmGradWeightsGrouped(e, st_dw, x_h(0), ws.p_act, ws.x_stride, dz1_tape(0), ws.p_dz, ws.dz_stride, R, B, H2, H2,
                                        reinterpret_cast<float*>(base + ws.off_partial_fc1), sums, grad + Fc1W(s, 0), BlockParams(s)));
-        // (with batch normalisation b2_k and the hidden bias got their gradients from the normalisation's backward pass)
-        sums.TowerBiases(s, colsum, colsum_rows, ws.colsum_slot_floats, grad, !bnorm);
+        // (with a normalisation b2_k and the hidden bias got their gradients from its backward pass)
+        sums.TowerBiases(s, colsum, colsum_rows, ws.colsum_slot_floats, grad, !normed);
         MGT_TRY(sums.Pass());
         if (cudaGetLastError() != cudaSuccess) return MGT_CUDA_FAILURE;
         for (uint32_t rb = R; rb > 0; --rb) {
@@ -2143,7 +2195,7 @@ mgt_status_t mgt_launch_mlp_loss_grad(mgt_engine_t* e, const mgt_mlp_shape_t* sh
     MGT_TRY(notify(HiddenWeight(s), (uint64_t)H1 * H2 + H2));
     if (!timer.Mark(profile ? &profile->hidden_backward_ms : nullptr)) return MGT_CUDA_FAILURE;
     MGT_TRY(notify(0, InputBias(s) + H1));
-    if (bnorm) MGT_TRY(notify(bn_base, 2ULL * (R + 1ULL) * H2));
+    if (normed) MGT_TRY(notify(bn_base, 2ULL * (R + 1ULL) * H2));
     return MGT_OK;
 }
 
@@ -2153,6 +2205,13 @@ mgt_status_t mgt_engine_set_train_options(mgt_engine_t* e, const mgt_train_optio
     if (options->loss_kind != MGT_LOSS_MSE && options->loss_kind != MGT_LOSS_CROSS_ENTROPY) return MGT_INVALID_CONFIG;
     if (options->batch_norm != 0 && !(options->bn_eps > 0.0f)) return MGT_INVALID_CONFIG;
     e->options = *options;
+    return MGT_OK;
+}
+
+mgt_status_t mgt_engine_set_layer_norm(mgt_engine_t* e, int32_t enabled, float eps) {
+    if (e == nullptr || (enabled != 0 && (!(eps > 0.0f) || !(eps <= 3.0e38f)))) return MGT_INVALID_CONFIG;
+    e->layer_norm = enabled != 0;
+    e->ln_eps = eps;
     return MGT_OK;
 }
 

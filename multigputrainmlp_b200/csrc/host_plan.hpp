@@ -37,6 +37,10 @@ struct TrainOptions {
     // vectors and the running statistics live beside the reference's files, and the exported weights have them folded in
     bool batch_norm = false;
     float bn_eps = 1.0e-5f, bn_momentum = 0.1f;
+    // layer normalisation in the same places (not both); its scale/shift vectors live beside the reference's files
+    bool layer_norm = false;
+    float ln_eps = 1.0e-5f;
+    float max_grad_norm = 0.0f;  // > 0: the averaged gradient is clipped to this norm before AdamW, a step without a finite norm is skipped
 };
 
 // Every flag takes exactly one value; unknown flags, missing values and unparsable values fail

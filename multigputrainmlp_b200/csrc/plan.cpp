@@ -88,6 +88,7 @@ bool ParseTrainOptions(int argc, const char* const* argv, TrainOptions* o) {
         {"--puzzle-json", text(&o->puzzle_json)}, {"--target-bin", text(&o->target_bin)},
         {"--operand-format", text(&o->operand_format)}, {"--loss", text(&o->loss)},
         {"--batch-norm", flag(&o->batch_norm)}, {"--bn-eps", f32(&o->bn_eps)}, {"--bn-momentum", f32(&o->bn_momentum)},
+        {"--layer-norm", flag(&o->layer_norm)}, {"--ln-eps", f32(&o->ln_eps)}, {"--max-grad-norm", f32(&o->max_grad_norm)},
     };
     for (int i = 1; i < argc; i += 2) {
         if (i + 1 >= argc) return false;
@@ -110,7 +111,9 @@ bool ValidateTrainOptions(const TrainOptions& o) {
     if (o.operand_format != "fp16" && o.operand_format != "bf16") return false;
     if (o.loss != "mse" && o.loss != "ce") return false;
     if (o.loss == "ce" && (o.output_dim < 2 || o.k_max > o.output_dim)) return false;  // one logit per walk depth
-    if ((o.loss == "ce" || o.operand_format == "bf16" || o.batch_norm) && !o.linear_fp16) return false;
+    if ((o.loss == "ce" || o.operand_format == "bf16" || o.batch_norm || o.layer_norm) && !o.linear_fp16) return false;
+    if (o.layer_norm && (o.batch_norm || !(o.ln_eps > 0.0f) || !(o.ln_eps <= 3.0e38f))) return false;
+    if (!(o.max_grad_norm >= 0.0f)) return false;
     if (o.batch_norm && (!(o.bn_eps > 0.0f) || !(o.bn_momentum >= 0.0f && o.bn_momentum <= 1.0f))) return false;
     return true;
 }

@@ -49,6 +49,7 @@ struct ExchangeContext {
     bool have_pending = false;
     uint64_t pending_offset = 0, pending_count = 0;
     bool failed = false;
+    bool average_only = false;  // clipping: the norm of the whole averaged gradient comes before any update
     bool have_early = false;  // the early-range hook already sent [early_begin, early_end)
     uint64_t early_begin = 0, early_end = 0;
 
@@ -59,7 +60,7 @@ struct ExchangeContext {
         if (!CUDA_OK(cudaEventRecord(ev, producer)) || !CUDA_OK(cudaStreamWaitEvent(comm_stream, ev, 0))) return false;
         while (count > 0) {
             const uint64_t chunk = whole ? count : std::min<uint64_t>(count, bucket_params);
-            if (exchange_only) {
+            if (exchange_only || average_only) {
                 const mgt_allreduce_config_t ar{world_size, global_rank, 0, chunk};
                 if (mgt_comm_allreduce_average(comm, &ar, grad + offset, comm_stream) != MGT_OK) return false;
             } else if (mgt_comm_allreduce_average_adamw(comm, offset, chunk, &adamw, w, w_half, m, v, comm_stream) != MGT_OK) {
@@ -132,7 +133,7 @@ mgt_status_t OnEarlyRange(void* user, uint32_t ready_id, uint64_t offset, uint64
     // The AdamW update moves 30 bytes per parameter through HBM and would fight the HBM-bound weight-gradient GEMMs that
     // run now; the NVLink exchange alone hardly touches local memory. So the update of this range is left for later,
     // unless an earlier early range is still waiting for its own (then this one takes the fused path).
-    const bool defer = ctx->early_update_after_backward && !ctx->have_deferred;
+    const bool defer = ctx->early_update_after_backward && !ctx->have_deferred && !ctx->average_only;
     if (!ctx->Flush(static_cast<cudaStream_t>(producer_stream)) || !ctx->LaunchRange(offset, count, static_cast<cudaStream_t>(producer_stream), true, defer)) {
         ctx->failed = true;
         return MGT_NCCL_FAILURE;
@@ -184,12 +185,34 @@ bool ReadBatchNormState(const std::string& checkpoint_dir, std::vector<float>* s
     return static_cast<bool>(data);
 }
 
+// Layer norm's scale/shift vectors, in checkpoint/ with their AdamW moments (three sections) and in weights/ alone: layer_norm.f32.bin and
+// a description beside the reference's files.
+bool WriteLayerNormState(const std::string& dir, std::initializer_list<const std::vector<float>*> sections, uint32_t layers, uint32_t width, float eps) {
+    std::ofstream data(dir + "/layer_norm.f32.bin", std::ios::binary | std::ios::trunc);
+    for (const std::vector<float>* section : sections)
+        data.write(reinterpret_cast<const char*>(section->data()), static_cast<std::streamsize>(section->size() * sizeof(float)));
+    std::ofstream man(dir + "/layer_norm.json", std::ios::trunc);
+    man << "{\n  \"format\": \"mgt_layer_norm_state_v1\",\n  \"layers\": " << layers << ",\n  \"width\": " << width << ",\n  \"eps\": " << eps
+        << ",\n  \"dtype\": \"f32\",\n  \"sections\": [\"scale_shift\"" << (sections.size() > 1 ? ", \"adam_m\", \"adam_v\"" : "")
+        << "],\n  \"section_floats\": " << (*sections.begin())->size()
+        << ",\n  \"layer_layout\": \"layer 0 = hidden layer, layer k+1 = residual block k; gamma[width], beta[width]\"\n}\n";
+    return static_cast<bool>(data) && static_cast<bool>(man);
+}
+bool ReadLayerNormState(const std::string& checkpoint_dir, std::vector<float>* scale_shift, std::vector<float>* m, std::vector<float>* v) {
+    std::ifstream data(checkpoint_dir + "/layer_norm.f32.bin", std::ios::binary);
+    if (!data) return false;
+    for (std::vector<float>* section : {scale_shift, m, v})
+        data.read(reinterpret_cast<char*>(section->data()), static_cast<std::streamsize>(section->size() * sizeof(float)));
+    return static_cast<bool>(data);
+}
+
 const char kUsage[] =
     "usage: mgt_native_train --output-dir DIR --steps N --device-id ID --world-size N --global-rank R --local-rank R "
     "[--batch-size N --k-min N --k-max N --hd1 N --hd2 N --nrd N --write-artifacts 0|1 --backward-profile 0|1 --overlap-allreduce 0|1 "
     "--input-grad-partial-chunks N --input-grad-positions-per-block N --input-grad-position-tile N --input-grad-fp16 0|1 --linear-fp16 0|1 "
     "--persistent-half-weights 0|1 --lt-workspace-bytes N --nccl-id-file PATH --resume-checkpoint DIR "
-    "--checkpoint-period-steps N --resume-step 0|1 --puzzle-json PATH --target-bin PATH --operand-format fp16|bf16 --loss mse|ce --batch-norm 0|1 --bn-eps X --bn-momentum X]\n";
+    "--checkpoint-period-steps N --resume-step 0|1 --puzzle-json PATH --target-bin PATH --operand-format fp16|bf16 --loss mse|ce --batch-norm 0|1 --bn-eps X --bn-momentum X "
+    "--layer-norm 0|1 --ln-eps X --max-grad-norm X]\n";
 
 }  // namespace
 
@@ -215,8 +238,8 @@ int main(int argc, char** argv) {
     const uint64_t P = plan.total_params;
     if (mgt_mlp_param_count(&shape) != P) return EXIT_FAILURE;
 
-    // trained floats on the device: the reference's parameters, then (with --batch-norm 1) the scale/shift vectors
-    const uint64_t NBN = opt.batch_norm ? mgt_bn_param_count(&shape) : 0;
+    // trained floats on the device: the reference's parameters, then (with --batch-norm 1 or --layer-norm 1) the scale/shift vectors
+    const uint64_t NBN = opt.batch_norm || opt.layer_norm ? mgt_bn_param_count(&shape) : 0;
     const uint64_t T = P + NBN;
     std::vector<float> weights(P), adam_m(P, 0.0f), adam_v(P, 0.0f);
     std::vector<float> bn_scale_shift(NBN, 0.0f), bn_m(NBN, 0.0f), bn_v(NBN, 0.0f), bn_running(NBN, 0.0f);
@@ -228,7 +251,11 @@ int main(int argc, char** argv) {
     InitialWeights(&weights);
     const bool resumed = !opt.resume_checkpoint.empty();
     if (resumed && !ReadCheckpoint(opt.resume_checkpoint, &weights, &adam_m, &adam_v)) return EXIT_FAILURE;
-    if (resumed && NBN != 0 && !ReadBatchNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v, &bn_running)) {
+    if (resumed && opt.layer_norm && !ReadLayerNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v)) {
+        std::cerr << "--layer-norm 1: " << opt.resume_checkpoint << "/layer_norm.f32.bin not found or too short\n";
+        return EXIT_FAILURE;
+    }
+    if (resumed && opt.batch_norm && !ReadBatchNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v, &bn_running)) {
         std::cerr << "--batch-norm 1: " << opt.resume_checkpoint << "/batch_norm.f32.bin not found or too short\n";
         return EXIT_FAILURE;
     }
@@ -262,7 +289,7 @@ int main(int argc, char** argv) {
     if (mgt_engine_create(static_cast<int32_t>(opt.device_id), &engine) != MGT_OK) return EXIT_FAILURE;
     const mgt_train_options_t train_options{opt.operand_format == "bf16" ? MGT_OPERAND_BF16 : MGT_OPERAND_FP16, opt.loss == "ce" ? MGT_LOSS_CROSS_ENTROPY : MGT_LOSS_MSE,
                                             opt.batch_norm ? 1 : 0, opt.bn_eps};
-    if (mgt_engine_set_train_options(engine, &train_options) != MGT_OK) return EXIT_FAILURE;
+    if (mgt_engine_set_train_options(engine, &train_options) != MGT_OK || mgt_engine_set_layer_norm(engine, opt.layer_norm ? 1 : 0, opt.ln_eps) != MGT_OK) return EXIT_FAILURE;
     // the communicator stands where the reference creates its NCCL context, also for one rank (tool:708-713)
     mgt_comm_t* comm = nullptr;
     if (mgt_comm_create(static_cast<int32_t>(opt.device_id), opt.world_size, opt.global_rank, opt.nccl_id_file.empty() ? nullptr : opt.nccl_id_file.c_str(), T, &comm) != MGT_OK) {
@@ -270,7 +297,7 @@ int main(int argc, char** argv) {
     }
     mgt_comm_t* stats_comm = nullptr;
     StatsContext stats_ctx;
-    if (NBN != 0 && opt.world_size > 1) {
+    if (opt.batch_norm && opt.world_size > 1) {
         const std::string stats_id = opt.nccl_id_file + ".bn";
         if (mgt_comm_create(static_cast<int32_t>(opt.device_id), opt.world_size, opt.global_rank, stats_id.c_str(), 2ULL * shape.hd2, &stats_comm) != MGT_OK) return EXIT_FAILURE;
         stats_ctx.comm = stats_comm;
@@ -285,11 +312,17 @@ int main(int argc, char** argv) {
     mgt_train_state_t *d_states = nullptr, *d_moves = nullptr, *d_target = nullptr;
     mgt_walk_meta_t* d_meta = nullptr;
     float* d_grad = mgt_comm_gradient_buffer(comm);  // peers map this buffer; with one rank it is plain device memory
-    const uint64_t ws_floats = mgt_mlp_loss_grad_workspace_floats_with_options(&shape, B, opt.input_grad_partial_chunks, opt.input_grad_fp16, opt.linear_fp16, &train_options);
+    const uint64_t ws_floats = opt.layer_norm ? mgt_mlp_loss_grad_workspace_floats_with_layer_norm(&shape, B, opt.input_grad_partial_chunks, opt.input_grad_fp16)
+                                              : mgt_mlp_loss_grad_workspace_floats_with_options(&shape, B, opt.input_grad_partial_chunks, opt.input_grad_fp16, opt.linear_fp16, &train_options);
+    const bool clipped = opt.max_grad_norm > 0.0f;
+    const mgt_tensor_t whole_gradient{d_grad, T, MGT_F32, 0};
+    const uint64_t norm_floats = clipped ? mgt_gradient_norm_workspace_floats(&whole_gradient, 1) : 0;
+    float *d_clip = nullptr, *d_norm_ws = nullptr;  // {norm, scale} of a step, scratch
     if (ws_floats == 0 || d_grad == nullptr) return EXIT_FAILURE;
     cudaStream_t compute = nullptr, comm_stream = nullptr;
     bool ok = CUDA_OK(cudaMalloc(&d_w, T * 4)) && (!(opt.linear_fp16 && opt.persistent_half_weights) || CUDA_OK(cudaMalloc(&d_w_half, T * 2))) &&
-              (NBN == 0 || CUDA_OK(cudaMalloc(&d_bn_running, NBN * 4))) &&
+              (!opt.batch_norm || CUDA_OK(cudaMalloc(&d_bn_running, NBN * 4))) &&
+              (!clipped || (CUDA_OK(cudaMalloc(&d_clip, 8)) && CUDA_OK(cudaMalloc(&d_norm_ws, norm_floats * 4)))) &&
               CUDA_OK(cudaMalloc(&d_labels, static_cast<uint64_t>(B) * opt.output_dim * 4)) &&
               (opt.output_dim == 1 || CUDA_OK(cudaMalloc(&d_walk_labels, static_cast<uint64_t>(B) * 4))) && CUDA_OK(cudaMalloc(&d_loss, 4)) &&
               CUDA_OK(cudaMalloc(&d_ws, ws_floats * 4)) && CUDA_OK(cudaMalloc(&d_m, T * 4)) && CUDA_OK(cudaMalloc(&d_v, T * 4)) &&
@@ -303,9 +336,10 @@ int main(int argc, char** argv) {
     if (!ok) return EXIT_FAILURE;
     if (NBN != 0) {
         ok = CUDA_OK(cudaMemcpy(d_w + P, bn_scale_shift.data(), NBN * 4, cudaMemcpyHostToDevice)) && CUDA_OK(cudaMemcpy(d_m + P, bn_m.data(), NBN * 4, cudaMemcpyHostToDevice)) &&
-             CUDA_OK(cudaMemcpy(d_v + P, bn_v.data(), NBN * 4, cudaMemcpyHostToDevice)) && CUDA_OK(cudaMemcpy(d_bn_running, bn_running.data(), NBN * 4, cudaMemcpyHostToDevice));
+             CUDA_OK(cudaMemcpy(d_v + P, bn_v.data(), NBN * 4, cudaMemcpyHostToDevice)) &&
+             (!opt.batch_norm || CUDA_OK(cudaMemcpy(d_bn_running, bn_running.data(), NBN * 4, cudaMemcpyHostToDevice)));
         if (!ok) return EXIT_FAILURE;
-        if (mgt_engine_set_batch_norm_state(engine, d_bn_running, opt.bn_momentum, opt.world_size, stats_comm != nullptr ? mgt_comm_gradient_buffer(stats_comm) : nullptr,
+        if (opt.batch_norm && mgt_engine_set_batch_norm_state(engine, d_bn_running, opt.bn_momentum, opt.world_size, stats_comm != nullptr ? mgt_comm_gradient_buffer(stats_comm) : nullptr,
                                             stats_comm != nullptr ? OnStatsExchange : nullptr, &stats_ctx) != MGT_OK) return EXIT_FAILURE;
     }
     if (d_w_half != nullptr && mgt_launch_float_to_half(d_w, T, d_w_half, compute) != MGT_OK) return EXIT_FAILURE;
@@ -313,13 +347,15 @@ int main(int argc, char** argv) {
     std::filesystem::create_directories(opt.output_dir);
     std::ofstream log(std::filesystem::path(opt.output_dir) / "train.log");
     std::ofstream profile(std::filesystem::path(opt.output_dir) / "profile.jsonl");
+    std::ofstream grad_norms;  // one row a step, beside the reference's files
+    if (clipped) grad_norms.open(std::filesystem::path(opt.output_dir) / "grad_norm.jsonl");
     cudaEvent_t ev_start, ev_walk, ev_backward, ev_allreduce, ev_stop, ev_comm_done, ev_early_done;
     if (!CUDA_OK(cudaEventCreate(&ev_start)) || !CUDA_OK(cudaEventCreate(&ev_walk)) || !CUDA_OK(cudaEventCreate(&ev_backward)) ||
         !CUDA_OK(cudaEventCreate(&ev_allreduce)) || !CUDA_OK(cudaEventCreate(&ev_stop)) ||
         !CUDA_OK(cudaEventCreateWithFlags(&ev_comm_done, cudaEventDisableTiming)) ||
         !CUDA_OK(cudaEventCreateWithFlags(&ev_early_done, cudaEventDisableTiming))) return EXIT_FAILURE;
     const bool overlap = comm_enabled && opt.overlap_allreduce && opt.world_size > 1;
-    const uint32_t expected_ranges = 2U * opt.nrd + 3U + (NBN != 0 ? 1U : 0U);  // batch norm: one more range, the scale/shift vectors
+    const uint32_t expected_ranges = 2U * opt.nrd + 3U + (NBN != 0 ? 1U : 0U);  // a normalisation: one more range, the scale/shift vectors
     std::vector<cudaEvent_t> ready_events;
     if (overlap) {
         ready_events.resize(expected_ranges + 1U, nullptr);
@@ -335,15 +371,17 @@ int main(int argc, char** argv) {
             !CUDA_OK(cudaMemcpy(adam_v.data(), d_v, P * 4, cudaMemcpyDeviceToHost))) return false;
         if (NBN != 0 && (!CUDA_OK(cudaMemcpy(bn_scale_shift.data(), d_w + P, NBN * 4, cudaMemcpyDeviceToHost)) || !CUDA_OK(cudaMemcpy(bn_m.data(), d_m + P, NBN * 4, cudaMemcpyDeviceToHost)) ||
                          !CUDA_OK(cudaMemcpy(bn_v.data(), d_v + P, NBN * 4, cudaMemcpyDeviceToHost)) ||
-                         !CUDA_OK(cudaMemcpy(bn_running.data(), d_bn_running, NBN * 4, cudaMemcpyDeviceToHost)))) return false;
+                         (opt.batch_norm && !CUDA_OK(cudaMemcpy(bn_running.data(), d_bn_running, NBN * 4, cudaMemcpyDeviceToHost))))) return false;
         if (with_weights) {
             // the weights/ files describe a network without normalisation: fold it in with the running statistics
             std::vector<float> exported = weights;
-            if (NBN != 0 && mgt_fold_batch_norm(&shape, exported.data(), bn_scale_shift.data(), bn_running.data(), opt.bn_eps) != MGT_OK) return false;
+            if (opt.batch_norm && mgt_fold_batch_norm(&shape, exported.data(), bn_scale_shift.data(), bn_running.data(), opt.bn_eps) != MGT_OK) return false;
             if (!WriteWeights(opt.output_dir, plan, exported)) return false;
+            if (opt.layer_norm && !WriteLayerNormState(opt.output_dir + "/weights", {&bn_scale_shift}, opt.nrd + 1U, shape.hd2, opt.ln_eps)) return false;
         }
         if (!WriteCheckpoint(opt.output_dir, plan, weights, adam_m, adam_v)) return false;
-        if (NBN != 0 && !WriteBatchNormState(opt.output_dir, bn_scale_shift, bn_m, bn_v, bn_running, opt.nrd + 1U, shape.hd2, opt.bn_eps, opt.bn_momentum)) return false;
+        if (opt.layer_norm && !WriteLayerNormState(opt.output_dir + "/checkpoint", {&bn_scale_shift, &bn_m, &bn_v}, opt.nrd + 1U, shape.hd2, opt.ln_eps)) return false;
+        if (opt.batch_norm && !WriteBatchNormState(opt.output_dir, bn_scale_shift, bn_m, bn_v, bn_running, opt.nrd + 1U, shape.hd2, opt.bn_eps, opt.bn_momentum)) return false;
         std::ofstream out(opt.output_dir + "/checkpoint/step.txt", std::ios::trunc);
         out << steps_done << "\n";
         return static_cast<bool>(out);
@@ -373,6 +411,7 @@ int main(int argc, char** argv) {
             exchange.w = d_w; exchange.w_half = d_w_half; exchange.m = d_m; exchange.v = d_v; exchange.grad = d_grad;
             exchange.world_size = opt.world_size; exchange.global_rank = opt.global_rank;
             exchange.early_done = ev_early_done;
+            exchange.average_only = clipped;
         }
         if (mgt_engine_set_early_range_hook(engine, overlap ? OnEarlyRange : nullptr, overlap ? &exchange : nullptr) != MGT_OK) return EXIT_FAILURE;
         mgt_backward_profile_t bw{};
@@ -396,14 +435,17 @@ int main(int argc, char** argv) {
             // the deferred update needs only its own range's exchange: it runs beside the tail of the exchange
             if (exchange.have_deferred && !CUDA_OK(cudaStreamWaitEvent(compute, ev_early_done, 0))) return EXIT_FAILURE;
             if (!exchange.UpdateDeferred(compute) || !CUDA_OK(cudaStreamWaitEvent(compute, ev_comm_done, 0))) return EXIT_FAILURE;
-            weights_updated = true;  // AdamW ran inside the exchange kernels
+            weights_updated = !clipped;  // AdamW ran inside the exchange kernels
         } else if (opt.world_size > 1) {
             const mgt_allreduce_config_t ar{opt.world_size, opt.global_rank, step, T};
             if (mgt_comm_allreduce_average(comm, &ar, d_grad, compute) != MGT_OK) return EXIT_FAILURE;
             overlap_chunks = 1;
         }
         if (!CUDA_OK(cudaEventRecord(ev_allreduce, compute))) return EXIT_FAILURE;
-        if (!weights_updated) {
+        if (!weights_updated && clipped) {
+            if (mgt_launch_gradient_norm(&whole_gradient, 1, opt.max_grad_norm, d_clip, nullptr, d_norm_ws, norm_floats, compute) != MGT_OK ||
+                mgt_launch_adamw_with_clip(&adamw, d_w, d_w_half, d_grad, d_clip, d_m, d_v, compute) != MGT_OK) return EXIT_FAILURE;
+        } else if (!weights_updated) {
             const mgt_status_t ad = d_w_half != nullptr ? mgt_launch_adamw_with_half_mirror(&adamw, d_w, d_w_half, d_grad, d_m, d_v, compute)
                                                         : mgt_launch_adamw(&adamw, d_w, d_grad, d_m, d_v, compute);
             if (ad != MGT_OK) return EXIT_FAILURE;
@@ -432,6 +474,15 @@ int main(int argc, char** argv) {
         std::copy(bwv, bwv + 7, rec.bw);
         log << StepLogLine(plan, rec);
         profile << StepProfileRow(plan, rec, overlap);
+        if (clipped) {
+            float clip[2];
+            if (!CUDA_OK(cudaMemcpy(clip, d_clip, 8, cudaMemcpyDeviceToHost))) return EXIT_FAILURE;
+            char row[96];  // (JSON has no word for a norm that is not finite)
+            const bool finite = clip[0] <= 3.402823466e38f;
+            if (finite) std::snprintf(row, sizeof(row), "{\"step\": %u, \"grad_norm\": %.9g, \"scale\": %.9g}\n", step, clip[0], clip[1]);
+            else std::snprintf(row, sizeof(row), "{\"step\": %u, \"grad_norm\": null, \"scale\": 0}\n", step);
+            grad_norms << row;
+        }
         const uint32_t done = step + 1U;
         if (opt.checkpoint_period_steps != 0 && done % opt.checkpoint_period_steps == 0 && done != first_step + opt.steps) {
             // every rank passes here at the same steps, whether or not it writes files itself
@@ -450,7 +501,7 @@ int main(int argc, char** argv) {
     for (cudaEvent_t ev : {ev_start, ev_walk, ev_backward, ev_allreduce, ev_stop, ev_comm_done, ev_early_done}) cudaEventDestroy(ev);
     for (void* p : {static_cast<void*>(d_target), static_cast<void*>(d_moves), static_cast<void*>(d_meta), static_cast<void*>(d_states), static_cast<void*>(d_v),
                     static_cast<void*>(d_m), static_cast<void*>(d_ws), static_cast<void*>(d_loss), static_cast<void*>(d_labels), static_cast<void*>(d_walk_labels),
-                    static_cast<void*>(d_w_half), static_cast<void*>(d_w), static_cast<void*>(d_bn_running)})
+                    static_cast<void*>(d_w_half), static_cast<void*>(d_w), static_cast<void*>(d_bn_running), static_cast<void*>(d_clip), static_cast<void*>(d_norm_ws)})
         if (p != nullptr) cudaFree(p);
     cudaStreamDestroy(comm_stream);
     cudaStreamDestroy(compute);
