@@ -47,32 +47,35 @@ F32, F16, BF16 = 0, 1, 2
 
 
 _torch = None
+_DTYPES = _CODES = _call = None
+
+
+class _Unfit(Exception):
+    """A tensor that cannot stand for what an argument asks for."""
 
 
 def _with_torch():
-    global _torch, _TYPES
+    """torch and the library, loaded on first use."""
+    global _torch, _DTYPES, _CODES, _call
     if _torch is None:
         import torch
-        _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        _DTYPES = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
+        _CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        _call = _lib.load()
         _torch = torch
     return _torch
 
 
-def _unfit(t, type_code, elements, device) -> bool:
-    """Whether a tensor cannot stand for `elements` of a type from its address on: another type, another device than `device` (the host
-    included), or too little behind the address. None and plain addresses are the library's to judge."""
-    if t is None or not hasattr(t, "data_ptr"):
-        return False
-    if _TYPES.get(t.dtype) != type_code or t.get_device() != device:
-        return True
-    if t.is_contiguous():
-        return t.numel() < elements
-    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < elements
-
-
-def _at(t):
-    """The address behind a tensor, or the address itself."""
-    return t.data_ptr() if hasattr(t, "data_ptr") else t
+def _address(t, type_code, elements, device):
+    """The address behind a tensor that holds `elements` of a type from there on. Another type, another device than `device` (the host
+    included) or too little behind the address raises _Unfit; None and plain addresses are the library's to judge."""
+    if t is None or isinstance(t, int):
+        return t
+    if t.dtype is not _DTYPES.get(type_code) or t.get_device() != device:
+        raise _Unfit
+    if (t.numel() if t.is_contiguous() else t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()) < elements:
+        raise _Unfit
+    return t.data_ptr()
 
 
 def _raw_stream(stream, device):
@@ -84,7 +87,7 @@ def _raw_stream(stream, device):
 
 def _current_device(stream):
     """The current device, of which tensors have to be. With plain addresses and a stream nothing is asked of torch's CUDA side."""
-    torch = _with_torch()
+    torch = _torch or _with_torch()
     return torch.cuda.current_device() if stream is None or torch.cuda.is_initialized() else None
 
 
@@ -361,14 +364,15 @@ def launch_float_to_half(device_values, count, device_half, stream=None) -> int:
 
 def launch_adamw_kernel_with_clip(config, device_weights, device_weights_half, device_grad, device_clip, device_m, device_v, stream=None) -> int:
     """mgt_launch_adamw_with_clip: the update of a gradient scaled by device_clip[1], skipped where the norm device_clip[0] is not finite
-    (what launch_gradient_norm leaves). device_weights_half may be None."""
+    (what launch_gradient_norm leaves). device_weights_half may be None. A tensor of another type, on another device than the
+    current one, or too small, is refused (1)."""
     n, d = config.param_count, _current_device(stream)
-    if (_unfit(device_weights, F32, n, d) or _unfit(device_grad, F32, n, d) or _unfit(device_m, F32, n, d) or _unfit(device_v, F32, n, d)
-            or _unfit(device_weights_half, F16, n, d) or _unfit(device_clip, F32, 2, d)):
+    try:
+        w, half = _address(device_weights, F32, n, d), _address(device_weights_half, F16, n, d)
+        grad, clip, m, v = _address(device_grad, F32, n, d), _address(device_clip, F32, 2, d), _address(device_m, F32, n, d), _address(device_v, F32, n, d)
+    except _Unfit:
         return 1
-    cfg = config.c()
-    return _lib.load().mgt_launch_adamw_with_clip(C.byref(cfg), _at(device_weights), _at(device_weights_half), _at(device_grad), _at(device_clip),
-                                                  _at(device_m), _at(device_v), _raw_stream(stream, d))
+    return _call.mgt_launch_adamw_with_clip(C.byref(config.c()), w, half, grad, clip, m, v, _raw_stream(stream, d))
 
 
 @dataclass(frozen=True)
@@ -406,10 +410,13 @@ def launch_layer_norm(config: LayerNormConfig, x, gamma, beta, y, mean=None, rst
     A tensor of another type, on another device than the current one, or too small, is refused (1)."""
     d = _current_device(stream)
     x_extent, y_extent, _ = config._extents
-    if (_unfit(x, config.x_type, x_extent, d) or _unfit(y, config.y_type, y_extent, d) or _unfit(gamma, F32, config.cols, d) or _unfit(beta, F32, config.cols, d)
-            or _unfit(mean, F32, config.rows, d) or _unfit(rstd, F32, config.rows, d)):
+    rows, cols = config.rows, config.cols
+    try:
+        x, y = _address(x, config.x_type, x_extent, d), _address(y, config.y_type, y_extent, d)
+        gamma, beta, mean, rstd = _address(gamma, F32, cols, d), _address(beta, F32, cols, d), _address(mean, F32, rows, d), _address(rstd, F32, rows, d)
+    except _Unfit:
         return 1
-    return _lib.load().mgt_launch_layer_norm(config._reference, _at(x), _at(gamma), _at(beta), _at(y), _at(mean), _at(rstd), _raw_stream(stream, d))
+    return _call.mgt_launch_layer_norm(config._reference, x, gamma, beta, y, mean, rstd, _raw_stream(stream, d))
 
 
 def layer_norm_backward_workspace_floats(config: LayerNormConfig) -> int:
@@ -420,12 +427,16 @@ def launch_layer_norm_backward(config: LayerNormConfig, dy, x, gamma, mean, rstd
     """mgt_launch_layer_norm_backward: dx, and the sums over the rows dgamma, dbeta and dbias (each may be None)."""
     d = _current_device(stream)
     x_extent, dy_extent, dx_extent = config._extents
-    if (_unfit(dy, config.y_type, dy_extent, d) or _unfit(x, config.x_type, x_extent, d) or _unfit(dx, config._dx_type, dx_extent, d)
-            or _unfit(gamma, F32, config.cols, d) or _unfit(dgamma, F32, config.cols, d) or _unfit(dbeta, F32, config.cols, d) or _unfit(dbias, F32, config.cols, d)
-            or _unfit(mean, F32, config.rows, d) or _unfit(rstd, F32, config.rows, d) or _unfit(workspace, F32, workspace_floats, d)):
+    rows, cols = config.rows, config.cols
+    try:
+        dy, x, dx = _address(dy, config.y_type, dy_extent, d), _address(x, config.x_type, x_extent, d), _address(dx, config._dx_type, dx_extent, d)
+        gamma, mean, rstd = _address(gamma, F32, cols, d), _address(mean, F32, rows, d), _address(rstd, F32, rows, d)
+        dgamma, dbeta, dbias = _address(dgamma, F32, cols, d), _address(dbeta, F32, cols, d), _address(dbias, F32, cols, d)
+        workspace = _address(workspace, F32, workspace_floats, d)
+    except _Unfit:
         return 1
-    return _lib.load().mgt_launch_layer_norm_backward(config._reference, _at(dy), _at(x), _at(gamma), _at(mean), _at(rstd), _at(dx), _at(dgamma), _at(dbeta),
-                                                      _at(dbias), _at(workspace), workspace_floats, _raw_stream(stream, d))
+    return _call.mgt_launch_layer_norm_backward(config._reference, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, dbias, workspace, workspace_floats,
+                                                _raw_stream(stream, d))
 
 
 class TensorList:
@@ -439,7 +450,7 @@ class TensorList:
         self._array = (_Tensor * max(1, self.count))()
         devices = set()
         for entry, t in zip(self._array, self.tensors):
-            kind = _TYPES.get(t.dtype)
+            kind = _CODES.get(t.dtype)
             if kind is None or not t.is_contiguous() or not t.is_cuda:
                 raise MgtError(1, "TensorList: dense CUDA tensors of float32, float16 or bfloat16")
             entry.data, entry.count, entry.type = t.data_ptr(), t.numel(), kind
@@ -451,22 +462,28 @@ class TensorList:
 
 
 def gradient_norm_workspace_floats(tensors: TensorList) -> int:
-    return _lib.load().mgt_gradient_norm_workspace_floats(tensors.pointer, tensors.count)
+    return _call.mgt_gradient_norm_workspace_floats(tensors.pointer, tensors.count)
 
 
 def launch_gradient_norm(tensors: TensorList, max_norm: float, result, tensor_norms, workspace, workspace_floats, stream=None) -> int:
     """mgt_launch_gradient_norm: result = {norm over all tensors, scale that brings it to max_norm at most}; tensor_norms (may be None) = the norm of each."""
     d = _current_device(stream)
-    if tensors.device != d or _unfit(result, F32, 2, d) or _unfit(tensor_norms, F32, tensors.count, d) or _unfit(workspace, F32, workspace_floats, d):
+    if tensors.device != d:
         return 1
-    return _lib.load().mgt_launch_gradient_norm(tensors.pointer, tensors.count, max_norm, _at(result), _at(tensor_norms), _at(workspace), workspace_floats,
-                                                _raw_stream(stream, d))
+    try:
+        result, norms, workspace = _address(result, F32, 2, d), _address(tensor_norms, F32, tensors.count, d), _address(workspace, F32, workspace_floats, d)
+    except _Unfit:
+        return 1
+    return _call.mgt_launch_gradient_norm(tensors.pointer, tensors.count, max_norm, result, norms, workspace, workspace_floats, _raw_stream(stream, d))
 
 
 def launch_clip_gradients(tensors: TensorList, result, out_tensors: TensorList | None = None, stream=None) -> int:
     """mgt_launch_clip_gradients: every element times result[1], in place or into out_tensors (same counts and types)."""
     d = _current_device(stream)
-    if tensors.device != d or _unfit(result, F32, 2, d) or (out_tensors is not None and (out_tensors.device != d or out_tensors.count != tensors.count)):
+    if tensors.device != d or (out_tensors is not None and (out_tensors.device != d or out_tensors.count != tensors.count)):
         return 1
-    return _lib.load().mgt_launch_clip_gradients(tensors.pointer, tensors.count, _at(result), out_tensors.pointer if out_tensors is not None else None,
-                                                 _raw_stream(stream, d))
+    try:
+        result = _address(result, F32, 2, d)
+    except _Unfit:
+        return 1
+    return _call.mgt_launch_clip_gradients(tensors.pointer, tensors.count, result, out_tensors.pointer if out_tensors is not None else None, _raw_stream(stream, d))

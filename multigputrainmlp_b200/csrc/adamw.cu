@@ -12,7 +12,9 @@ namespace {
 constexpr uint32_t kAdamWThreads = 128;
 constexpr uint64_t kOverlapParams = 8ULL << 20;  // a longer update does not notice the gap before it, and its CTAs crowd what still runs
 
-// kClip: the gradient is scaled by clip[1] on its way, and a norm clip[0] that is not finite leaves everything as it is.
+// kClip: the gradient is scaled by clip[1] on its way, and a norm clip[0] that is not finite leaves everything as it is. The pass over the
+// gradient that found the norm has just left the end of it in L2: so this one begins at the end, and reads what nobody reads again
+// soon (weights, moments) without keeping it there. 15.5 M parameters with norm and mirror 92.0 -> 89.3 us, 40.2 M without mirror 220 -> 208.
 template <bool kMirror, bool kClip>
 __global__ void __launch_bounds__(kAdamWThreads)
 AdamWKernel(mgt_adamw_config_t config, float* __restrict__ w, __half* __restrict__ w_half, const float* __restrict__ g,
@@ -22,21 +24,25 @@ AdamWKernel(mgt_adamw_config_t config, float* __restrict__ w, __half* __restrict
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
     mgt::dependent_begin();
     float scale = 1.0f;
+    bool skip = false;
     if (kClip) {
         const float* c = mgt::after_begin(clip);
-        if (!(c[0] <= 3.402823466e38f)) return;
+        skip = !(c[0] <= 3.402823466e38f);
         scale = c[1];
     }
-    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n4; i += stride) {
-        float4 wv = reinterpret_cast<float4*>(w)[i];
+    const uint32_t block = kClip ? gridDim.x - 1U - blockIdx.x : blockIdx.x;
+    auto load = [](const float* p, uint64_t i) { return kClip ? __ldcs(reinterpret_cast<const float4*>(p) + i) : reinterpret_cast<const float4*>(p)[i]; };
+    for (uint64_t i = static_cast<uint64_t>(block) * blockDim.x + threadIdx.x; i < n4; i += stride) {
+        float4 wv = load(w, i);
         float4 gv = reinterpret_cast<const float4*>(g)[i];
-        float4 mv = reinterpret_cast<float4*>(m)[i];
-        float4 vv = reinterpret_cast<float4*>(v)[i];
+        float4 mv = load(m, i);
+        float4 vv = load(v, i);
         if (kClip) gv = make_float4(__fmul_rn(gv.x, scale), __fmul_rn(gv.y, scale), __fmul_rn(gv.z, scale), __fmul_rn(gv.w, scale));
         wv.x = mgt::AdamWUpdateOne(sc, wv.x, gv.x, &mv.x, &vv.x);
         wv.y = mgt::AdamWUpdateOne(sc, wv.y, gv.y, &mv.y, &vv.y);
         wv.z = mgt::AdamWUpdateOne(sc, wv.z, gv.z, &mv.z, &vv.z);
         wv.w = mgt::AdamWUpdateOne(sc, wv.w, gv.w, &mv.w, &vv.w);
+        if (kClip && skip) return;  // (here, so that the loads above do not wait for the norm)
         reinterpret_cast<float4*>(w)[i] = wv;
         reinterpret_cast<float4*>(m)[i] = mv;
         reinterpret_cast<float4*>(v)[i] = vv;
@@ -52,7 +58,7 @@ AdamWKernel(mgt_adamw_config_t config, float* __restrict__ w, __half* __restrict
     // tail (param_count % 4)
     const uint64_t tail0 = n4 << 2;
     const uint64_t t = tail0 + static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (t < config.param_count) {
+    if (t < config.param_count && !(kClip && skip)) {
         float mm = m[t], vv = v[t];
         const float nw = mgt::AdamWUpdateOne(sc, w[t], kClip ? __fmul_rn(g[t], scale) : g[t], &mm, &vv);
         w[t] = nw;

@@ -16,8 +16,9 @@
 namespace {
 
 constexpr uint32_t kThreads = 256, kFinishThreads = 1024;
-constexpr uint64_t kLeastChunk = 4096;  // elements: sixteen a thread
-constexpr uint32_t kWantedChunks = 148 * 8;
+constexpr int kUnroll = 4;  // 16-byte loads of a thread in flight
+constexpr uint32_t kLeastChunkBytes = 16384;  // four such loads a thread: more chunks than the chip holds CTAs, so that none waits long for a last one
+constexpr uint32_t kMostChunks = 4000;  // of whole length: longer chunks beyond, so that their sums fit into the shared memory of a CTA
 
 // Tensors of a call as the kernels get them: where a tensor begins in the line of chunks, and its type in the top bits of its count.
 template <uint32_t kMost>
@@ -68,23 +69,23 @@ __device__ __forceinline__ uint64_t HeadCount(const T* p, uint64_t n) {
 template <class T>
 __device__ double SumOfSquares(const T* p, uint64_t n) {
     const uint64_t head = HeadCount(p, n);
-    double s = 0.0;
-    auto add = [&](float f) {
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    auto add = [&](float f, uint32_t j) {
         const double d = static_cast<double>(f);
-        s = fma(d, d, s);
+        s[j & 3U] = fma(d, d, s[j & 3U]);
     };
-    if (threadIdx.x < head) add(Vec<T>::One(p[threadIdx.x]));
+    if (threadIdx.x < head) add(Vec<T>::One(p[threadIdx.x]), 0);
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
-    const uint64_t vectors = (n - head) / Vec<T>::kCount;
-#pragma unroll 4
-    for (uint64_t i = threadIdx.x; i < vectors; i += kThreads) {
+    const uint32_t vectors = static_cast<uint32_t>((n - head) / Vec<T>::kCount);
+#pragma unroll kUnroll
+    for (uint32_t i = threadIdx.x; i < vectors; i += kThreads) {
         const uint4 w = body[i];
 #pragma unroll
-        for (uint32_t j = 0; j < Vec<T>::kCount; ++j) add(Vec<T>::Get(w, j));
+        for (uint32_t j = 0; j < Vec<T>::kCount; ++j) add(Vec<T>::Get(w, j), j);
     }
     const uint64_t at = head + vectors * Vec<T>::kCount + threadIdx.x;
-    if (at < n) add(Vec<T>::One(p[at]));
-    return s;
+    if (at < n) add(Vec<T>::One(p[at]), 0);
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 template <class T>
@@ -98,13 +99,13 @@ __device__ void Scale(const T* p, T* out, uint64_t n, float scale, bool zero) {
     if (threadIdx.x < head) out[threadIdx.x] = Vec<T>::To(scaled(Vec<T>::One(p[threadIdx.x])));
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
     uint4* to = reinterpret_cast<uint4*>(out + head);
-    const uint64_t vectors = (n - head) / Vec<T>::kCount;
-#pragma unroll 4
-    for (uint64_t i = threadIdx.x; i < vectors; i += kThreads) {
+    const uint32_t vectors = static_cast<uint32_t>((n - head) / Vec<T>::kCount);
+#pragma unroll kUnroll
+    for (uint32_t i = threadIdx.x; i < vectors; i += kThreads) {
         uint4 w = body[i];
 #pragma unroll
         for (uint32_t j = 0; j < Vec<T>::kCount; ++j) Vec<T>::Put(w, j, scaled(Vec<T>::Get(w, j)));
-        to[i] = w;
+        __stcs(to + i, w);
     }
     const uint64_t at = head + vectors * Vec<T>::kCount + threadIdx.x;
     if (at < n) out[at] = Vec<T>::To(scaled(Vec<T>::One(p[at])));
@@ -131,11 +132,11 @@ template <uint32_t kMost>
 __global__ void __launch_bounds__(kThreads)
 ChunkSquaresKernel(const __grid_constant__ Table<kMost> t, double* __restrict__ partial) {
     __shared__ double warps[kThreads / 32U];
-    mgt::dependent_begin();
     const uint32_t tensor = TensorOf(t, blockIdx.x);
     const uint64_t begin = static_cast<uint64_t>(blockIdx.x - t.first_chunk[tensor]) * t.chunk, all = t.count[tensor] & kCountMask;
     const uint64_t n = all - begin < t.chunk ? all - begin : t.chunk;
     const int32_t type = static_cast<int32_t>(t.count[tensor] >> kTypeShift);
+    mgt::dependent_begin();
     double s = type == MGT_F32    ? SumOfSquares(static_cast<const float*>(t.data[tensor]) + begin, n)
                : type == MGT_F16 ? SumOfSquares(static_cast<const __half*>(t.data[tensor]) + begin, n)
                                  : SumOfSquares(static_cast<const __nv_bfloat16*>(t.data[tensor]) + begin, n);
@@ -153,11 +154,11 @@ ChunkSquaresKernel(const __grid_constant__ Table<kMost> t, double* __restrict__ 
 template <uint32_t kMost>
 __global__ void __launch_bounds__(kFinishThreads)
 FinishNormKernel(const __grid_constant__ Table<kMost> t, const double* __restrict__ partial, float max_norm, float* __restrict__ result, float* __restrict__ norms) {
-    __shared__ double chunks[kWantedChunks + kMost], squares[kMost], warps[kFinishThreads / 32U];
+    __shared__ double chunks[kMostChunks + kMost], squares[kMost], warps[kFinishThreads / 32U];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31U, all = t.first_chunk[t.tensors];
     mgt::dependent_begin();
 #pragma unroll
-    for (uint32_t c = threadIdx.x; c < kWantedChunks + kMost; c += kFinishThreads)
+    for (uint32_t c = threadIdx.x; c < kMostChunks + kMost; c += kFinishThreads)
         if (c < all) chunks[c] = partial[c];
     __syncthreads();
     for (uint32_t k = warp; k < t.tensors; k += kFinishThreads / 32U) {
@@ -191,14 +192,15 @@ FinishNormKernel(const __grid_constant__ Table<kMost> t, const double* __restric
 template <uint32_t kMost>
 __global__ void __launch_bounds__(kThreads)
 ScaleKernel(const __grid_constant__ Table<kMost> t, const __grid_constant__ Outputs<kMost> out, const float* __restrict__ result, bool in_place) {
+    const uint32_t chunk = gridDim.x - 1U - blockIdx.x;  // from the end, which the pass for the norm has left in L2
+    const uint32_t tensor = TensorOf(t, chunk);
+    const uint64_t begin = static_cast<uint64_t>(chunk - t.first_chunk[tensor]) * t.chunk, all = t.count[tensor] & kCountMask;
+    const uint64_t n = all - begin < t.chunk ? all - begin : t.chunk;
+    const int32_t type = static_cast<int32_t>(t.count[tensor] >> kTypeShift);
     mgt::dependent_begin();
     const float norm = result[0], scale = result[1];
     const bool zero = !(norm <= 3.402823466e38f);
     if (in_place && !zero && scale == 1.0f) return;  // every product is the value that is there
-    const uint32_t tensor = TensorOf(t, blockIdx.x);
-    const uint64_t begin = static_cast<uint64_t>(blockIdx.x - t.first_chunk[tensor]) * t.chunk, all = t.count[tensor] & kCountMask;
-    const uint64_t n = all - begin < t.chunk ? all - begin : t.chunk;
-    const int32_t type = static_cast<int32_t>(t.count[tensor] >> kTypeShift);
     if (type == MGT_F32) Scale(static_cast<const float*>(t.data[tensor]) + begin, static_cast<float*>(out.data[tensor]) + begin, n, scale, zero);
     else if (type == MGT_F16) Scale(static_cast<const __half*>(t.data[tensor]) + begin, static_cast<__half*>(out.data[tensor]) + begin, n, scale, zero);
     else Scale(static_cast<const __nv_bfloat16*>(t.data[tensor]) + begin, static_cast<__nv_bfloat16*>(out.data[tensor]) + begin, n, scale, zero);
@@ -219,9 +221,13 @@ bool ValidTensors(const mgt_tensor_t* tensors, uint32_t count) {
 }
 uint64_t ChunkOf(const mgt_tensor_t* tensors, uint32_t count) {
     uint64_t total = 0;
-    for (uint32_t i = 0; i < count; ++i) total += tensors[i].count;
-    const uint64_t chunk = (total / kWantedChunks + 1023ULL) / 1024ULL * 1024ULL;
-    return chunk < kLeastChunk ? kLeastChunk : chunk;
+    uint32_t bytes = 2;  // of the widest type
+    for (uint32_t i = 0; i < count; ++i) {
+        total += tensors[i].count;
+        if (tensors[i].type == MGT_F32) bytes = 4;
+    }
+    const uint64_t chunk = (total / kMostChunks + 1024ULL) / 1024ULL * 1024ULL;
+    return chunk < kLeastChunkBytes / bytes ? kLeastChunkBytes / bytes : chunk;
 }
 uint32_t Chunks(const mgt_tensor_t* tensors, uint32_t count, uint64_t chunk) {
     uint64_t n = 0;
