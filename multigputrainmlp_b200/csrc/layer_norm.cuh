@@ -309,7 +309,7 @@ __device__ __forceinline__ float SumOf(const Held<E>& v) {
     return s.x + s.y;
 }
 // ---- host side: how a row is cut
-constexpr uint32_t kMostLanes = 512, kElements = 16;
+constexpr uint32_t kElements = 16;  // that a thread holds of a row at most
 struct Cut {
     uint32_t nv;         // packs a thread
     uint32_t lanes, threads;
@@ -321,10 +321,10 @@ inline uint32_t PowerOfTwo(uint32_t n) {
     return p;
 }
 // As few lanes a row as can hold it, which makes the reductions short, or more where the rows are too few to fill the chip's threads.
-inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v) {
+inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v, uint32_t most_lanes) {
     const uint32_t packs = (cols - 1U) / v + 1U, most = kElements / v;
     Cut c{1, 1, 256, false};
-    if (packs > most * kMostLanes) {
+    if (packs > most * most_lanes) {
         c.stream = true;
         return c;
     }

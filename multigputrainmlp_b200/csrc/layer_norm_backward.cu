@@ -8,9 +8,8 @@ namespace mgt {
 namespace ln {
 namespace {
 
-constexpr uint32_t kSums = 3;
+constexpr uint32_t kSums = 3, kMostLanes = 512;
 constexpr uint32_t kSms = 148, kMostCtas = 2 * kSms;  // partial rows at most: two CTAs an SM
-constexpr int kMostShared = 200 << 10;
 constexpr uint32_t kColumnSlices = 37;  // widest rows: slices of the batch that the column sums are taken over
 
 inline __host__ __device__ uint32_t PartialPitch(uint32_t cols) { return (cols + 3U) / 4U * 4U; }
@@ -205,22 +204,37 @@ StreamColumnsKernel(const Backward a, const float2* means, uint32_t rows_each) {
     float gamma[V], sums[kSums][V] = {};
 #pragma unroll
     for (int j = 0; j < V; ++j) gamma[j] = a.gamma != nullptr ? a.gamma[c + j] : 1.0f;
-#pragma unroll 4
-    for (uint64_t row = r0; row < r1; ++row) {
-        const Pack<Tdy, V> pd = LoadPack<Tdy, V>(static_cast<const Tdy*>(a.dy) + row * a.dy_pitch + c);
-        const Pack<Tx, V> px = LoadPack<Tx, V>(static_cast<const Tx*>(a.x) + row * a.x_pitch + c);
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        const float2 m = means[row];
-        Pack<Tdx, V> out;
+    // four rows at once: the compiler keeps a load behind the store before it (dx may be dy or x)
+    for (uint64_t first = r0; first < r1; first += 4U) {
+        Pack<Tdy, V> pd[4];
+        Pack<Tx, V> px[4];
+        float mean[4], rstd[4];
+        float2 m[4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float d = ToFloat(pd.v[j]), xhat = (ToFloat(px.v[j]) - mean) * rstd, o = rstd * (d * gamma[j] - m.x - xhat * m.y);
-            sums[0][j] += d * xhat;
-            sums[1][j] += d;
-            sums[2][j] += o;
-            out.v[j] = FromFloat<Tdx>(o);
+        for (uint32_t i = 0; i < 4U; ++i) {
+            const uint64_t row = first + i;
+            if (row >= r1) continue;
+            pd[i] = LoadPack<Tdy, V>(static_cast<const Tdy*>(a.dy) + row * a.dy_pitch + c);
+            px[i] = LoadPack<Tx, V>(static_cast<const Tx*>(a.x) + row * a.x_pitch + c);
+            mean[i] = a.mean[row];
+            rstd[i] = a.rstd[row];
+            m[i] = means[row];
         }
-        StorePack<Tdx, V>(static_cast<Tdx*>(a.dx) + row * a.dx_pitch + c, out);
+#pragma unroll
+        for (uint32_t i = 0; i < 4U; ++i) {
+            const uint64_t row = first + i;
+            if (row >= r1) continue;
+            Pack<Tdx, V> out;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = ToFloat(pd[i].v[j]), xhat = (ToFloat(px[i].v[j]) - mean[i]) * rstd[i], o = rstd[i] * (d * gamma[j] - m[i].x - xhat * m[i].y);
+                sums[0][j] += d * xhat;
+                sums[1][j] += d;
+                sums[2][j] += o;
+                out.v[j] = FromFloat<Tdx>(o);
+            }
+            StorePack<Tdx, V>(static_cast<Tdx*>(a.dx) + row * a.dx_pitch + c, out);
+        }
     }
     const uint32_t pitch = PartialPitch(a.cols);
     float* partial = a.partial + static_cast<uint64_t>(blockIdx.y) * kSums * pitch;
@@ -241,10 +255,10 @@ mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint64_t want = (static_cast<uint64_t>(a.rows) + groups - 1U) / groups;
     const uint32_t most = kSms * F::kCtas, ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
-    const uint32_t rings = F::kGammaBytes + F::RingDy::kBytes + F::RingX::kBytes;
-    const uint32_t sums = groups > 1U ? groups * a.cols * 4U : 0U, smem = rings > sums ? rings : sums;
+    constexpr uint32_t smem = F::kGammaBytes + F::RingDy::kBytes + F::RingX::kBytes;
+    static_assert(smem >= F::E * F::kThreads * 4U, "the sums of all groups, a float a column of each");
     static std::atomic<uint64_t> allowed{0};
-    if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, F>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
+    if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, F>, allowed, smem)) return MGT_CUDA_FAILURE;
     Launch(BackwardKernel<Tdy, Tx, Tdx, F>, ctas, cut.threads, smem, on, a);
     ++*launches;
     if (ctas > 1U && (a.sums[0] != nullptr || a.sums[1] != nullptr || a.sums[2] != nullptr)) SumPartialRows(a, ctas, on, launches);
@@ -252,7 +266,7 @@ mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
 }
 template <class Tdy, class Tx, class Tdx, int V>
 mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
-    const Cut cut = CutRow(a.rows, a.cols, V);
+    const Cut cut = CutRow(a.rows, a.cols, V, kMostLanes);
     if (cut.stream) {
         float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(a.cols));
         Launch(StreamMeansKernel<Tdy, Tx, V>, a.rows < 2U * kSms ? a.rows : 2U * kSms, 1024, 0, on, a, means);

@@ -17,8 +17,8 @@ __device__ __forceinline__ Moments Finish(float first, const float (&sums)[2], f
     return {first + shift, shift, r * fmaf(-0.5f * v * r, r, 1.5f)};  // one Newton step: to an ulp, at a tenth of a root's and a division's price
 }
 
-template <class Tx, class Lay>
-constexpr int kDepth = Lay::V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : Lay::E * sizeof(Tx) >= 64 ? 3 : Lay::E * sizeof(Tx) >= 32 ? 5 : 8;
+template <class Tx, class Lay, int kThreads>
+constexpr int kDepth = kThreads > 512 ? (sizeof(Tx) == 2 ? 2 : 1) : Lay::V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : Lay::E * sizeof(Tx) >= 64 ? 3 : Lay::E * sizeof(Tx) >= 32 ? 5 : 8;
 template <class Lay, int kThreads>
 constexpr uint32_t kCtas = kThreads > 256 ? 1 : Lay::V == 1 && Lay::E > 8 ? 2 : 3;  // an SM (single columns take more registers)
 
@@ -27,9 +27,10 @@ constexpr uint32_t kCtas = kThreads > 256 ? 1 : Lay::V == 1 && Lay::E > 8 ? 2 : 
 template <class Tx, class Ty, class Lay, int kThreads, bool kTower>
 __global__ void __launch_bounds__(kThreads, kCtas<Lay, kThreads>)
 ForwardKernel(const Forward a) {
-    extern __shared__ __align__(16) char memory[];
+    extern __shared__ __align__(16) char memory[];  // the ring, then gamma and beta where registers have no room for them
     __shared__ float buffer[2 * 2 * (kThreads / 32)];
-    constexpr int V = Lay::V, E = Lay::E, D = kDepth<Tx, Lay>, kPairs = Held<E>::kPairs;
+    constexpr bool kFar = kThreads > 512;
+    constexpr int V = Lay::V, E = Lay::E, D = kDepth<Tx, Lay, kThreads>, kPairs = Held<E>::kPairs;
     Group g = MakeGroup(a.lanes, buffer);
     const Share share = MakeShare(g, a.rows);
     const Lay lay(g, a.cols);
@@ -46,8 +47,18 @@ ForwardKernel(const Forward a) {
         CopiesEnd();
     }
     Held<E> gamma, beta, v;
-    LoadColumns(gamma, lay, a.gamma, 1.0f);
-    LoadColumns(beta, lay, a.beta, 0.0f);
+    float2* far = reinterpret_cast<float2*>(memory + Ring<Tx, Lay, kThreads, D>::kBytes) + threadIdx.x;
+    if constexpr (kFar) {
+        LoadColumns(v, lay, a.gamma, 1.0f);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) far[k * kThreads] = v.pair[k];
+        LoadColumns(v, lay, a.beta, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) far[(kPairs + k) * kThreads] = v.pair[k];
+    } else {
+        LoadColumns(gamma, lay, a.gamma, 1.0f);
+        LoadColumns(beta, lay, a.beta, 0.0f);
+    }
     uint32_t slot = 0, row = share.first;
     for (uint32_t t = 0; t < share.turns; ++t) {
         const bool in = t < share.mine;
@@ -86,7 +97,8 @@ ForwardKernel(const Forward a) {
             }
             const float2 rstd = Both(mo.rstd), off = Both(-mo.shift * mo.rstd);
 #pragma unroll
-            for (int k = 0; k < kPairs; ++k) v.pair[k] = Fma2(Fma2(v.pair[k], rstd, off), gamma.pair[k], beta.pair[k]);
+            for (int k = 0; k < kPairs; ++k)
+                v.pair[k] = Fma2(Fma2(v.pair[k], rstd, off), kFar ? far[k * kThreads] : gamma.pair[k], kFar ? far[(kPairs + k) * kThreads] : beta.pair[k]);
             lay.Each([&](int i, bool has) {
                 if (!has) return;
                 const uint32_t at = lay.Offset(i);
@@ -105,7 +117,8 @@ ForwardKernel(const Forward a) {
     }
 }
 
-// Rows wider than the registers of a CTA: a CTA a row, which it reads three times (from its L1 and L2 after the first).
+// Rows wider than the registers of a CTA: a CTA a row, which it reads three times (from its L1 and L2 after the first), four packs at once
+// (the compiler keeps a load behind the store before it: y may be x).
 template <class Tx, class Ty, int V>
 __global__ void __launch_bounds__(1024)
 StreamForwardKernel(const Forward a) {
@@ -143,19 +156,25 @@ StreamForwardKernel(const Forward a) {
             if (a.mean != nullptr) a.mean[row] = mo.mean;
             if (a.rstd != nullptr) a.rstd[row] = mo.rstd;
         }
-#pragma unroll 2
-        for (uint32_t c = threadIdx.x * V; c < a.cols; c += step) {
-            const Pack<Tx, V> p = LoadPack<Tx, V>(x + c);
-            Pack<Ty, V> out;
+        for (uint32_t c0 = threadIdx.x * V; c0 < a.cols; c0 += 4U * step) {
+            Pack<Tx, V> p[4];
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                out.v[j] = FromFloat<Ty>(((ToFloat(p.v[j]) - m) - mo.shift) * mo.rstd * (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) + (a.beta != nullptr ? a.beta[c + j] : 0.0f));
-            StorePack<Ty, V>(y + c, out);
+            for (uint32_t i = 0; i < 4U; ++i)
+                if (c0 + i * step < a.cols) p[i] = LoadPack<Tx, V>(x + c0 + i * step);
+#pragma unroll
+            for (uint32_t i = 0; i < 4U; ++i) {
+                const uint32_t c = c0 + i * step;
+                if (c >= a.cols) continue;
+                Pack<Ty, V> out;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    out.v[j] = FromFloat<Ty>(((ToFloat(p[i].v[j]) - m) - mo.shift) * mo.rstd * (a.gamma != nullptr ? a.gamma[c + j] : 1.0f) + (a.beta != nullptr ? a.beta[c + j] : 0.0f));
+                StorePack<Ty, V>(y + c, out);
+            }
         }
     }
 }
 
-constexpr int kMostShared = 110 << 10;
 
 template <class Tx, class Ty, class Lay, int kThreads, bool kTower>
 mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
@@ -163,8 +182,8 @@ mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
     const uint64_t want = (static_cast<uint64_t>(a.rows) + rows - 1U) / rows;
     a.lanes = cut.lanes;
     static std::atomic<uint64_t> allowed{0};
-    const uint32_t smem = Ring<Tx, Lay, kThreads, kDepth<Tx, Lay>>::kBytes;
-    if (!AllowShared(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, allowed, kMostShared)) return MGT_CUDA_FAILURE;
+    constexpr uint32_t smem = Ring<Tx, Lay, kThreads, kDepth<Tx, Lay, kThreads>>::kBytes + (kThreads > 512 ? Lay::E * kThreads * 8U : 0U);
+    if (!AllowShared(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, allowed, smem)) return MGT_CUDA_FAILURE;
     const uint32_t most = 148U * kCtas<Lay, kThreads>;
     Launch(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, static_cast<uint32_t>(want < most ? want : most), cut.threads, smem, on, a);
     return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
@@ -172,7 +191,7 @@ mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
 // (packs that a kernel has room for and the row does not have lie beyond its end)
 template <class Tx, class Ty, int V, bool kTower>
 mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
-    const Cut cut = CutRow(a.rows, a.cols, V);
+    const Cut cut = CutRow(a.rows, a.cols, V, 1024);
     constexpr int kMost = kElements / V;
     if (cut.stream || (kTower && cut.threads > 256U)) {
         if constexpr (kTower) return MGT_INVALID_CONFIG;  // (no tower is that wide)
@@ -180,7 +199,10 @@ mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
     if constexpr (!kTower)
-        if (cut.threads > 256U) return Run<Tx, Ty, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512, false>(a, cut, on);
+        if (cut.threads > 256U) {
+            using Lay = Layout<V, kMost, 32, V == 1 ? 8 : 0>;
+            return cut.threads > 512U ? Run<Tx, Ty, Lay, 1024, false>(a, cut, on) : Run<Tx, Ty, Lay, 512, false>(a, cut, on);
+        }
     if constexpr (V == 1) {
         return SingleColumns(cut, [&](auto tag) { return Run<Tx, Ty, typename decltype(tag)::type, 256, kTower>(a, cut, on); });
     } else {
