@@ -35,6 +35,24 @@ struct LaunchOn {
     operator cudaStream_t() const { return stream; }
 };
 
+// Clusters of neighbouring CTAs of a one-dimensional grid.
+template <class... Params, class... Args>
+inline cudaError_t LaunchClusters(uint32_t cluster, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, LaunchOn on, Args&&... args) {
+    cudaLaunchAttribute attrs[2]{};
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = cluster;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = smem;
+    config.stream = on.stream;
+    config.attrs = attrs;
+    config.numAttrs = on.overlap ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+}
 template <class... Params, class... Args>
 inline cudaError_t Launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, LaunchOn on, Args&&... args) {
     cudaLaunchAttribute attr{};

@@ -145,10 +145,11 @@ __device__ __forceinline__ void Reduce(Group& g, float (&v)[N]) {
 struct Share {
     uint32_t first, stride, mine, turns;
 };
-__device__ __forceinline__ Share MakeShare(const Group& g, uint32_t rows) {
+// cta of ctas: CTAs that share a row count as one.
+__device__ __forceinline__ Share MakeShare(const Group& g, uint32_t rows, uint32_t cta, uint32_t ctas) {
     Share s;
-    s.first = blockIdx.x * g.count + g.index;
-    s.stride = gridDim.x * g.count;
+    s.first = cta * g.count + g.index;
+    s.stride = ctas * g.count;
     const uint32_t least = g.lanes < 32U ? s.first - (g.index & (32U / g.lanes - 1U)) : s.first;
     s.mine = s.first < rows ? (rows - 1U - s.first) / s.stride + 1U : 0U;
     s.turns = least < rows ? (rows - 1U - least) / s.stride + 1U : 0U;
@@ -213,14 +214,14 @@ struct Ring {
     char* slots;                // of this thread (V > 1) or stretch
     uintptr_t least, most;      // the matrix (V = 1)
 
-    __device__ __forceinline__ Ring(const void* base, uint64_t pitch, uint32_t rows, char* memory, const Share& share, const Lay& lay) {
-        next = static_cast<const T*>(base) + share.first * pitch + (V > 1 ? lay.base : lay.begin);
+    __device__ __forceinline__ Ring(const T* base, uint64_t pitch, uint32_t rows, char* memory, const Share& share, const Lay& lay) {
+        next = base + share.first * pitch + (V > 1 ? lay.base : lay.begin);
         step = share.stride * pitch;
         slots = memory + (V > 1 ? threadIdx.x * kPackBytes : threadIdx.x / Lay::L * kLineBytes);
         now = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(next));
         now_step = static_cast<uint32_t>(step * sizeof(T));
         least = reinterpret_cast<uintptr_t>(base);
-        most = reinterpret_cast<uintptr_t>(static_cast<const T*>(base) + (rows - 1ULL) * pitch + lay.cols);
+        most = reinterpret_cast<uintptr_t>(base + (rows - 1ULL) * pitch + lay.cols);
     }
     __device__ __forceinline__ char* Slot(uint32_t turn, int i) const {
         if constexpr (V > 1) return slots + (turn * NV + i) * (kThreads * kPackBytes);

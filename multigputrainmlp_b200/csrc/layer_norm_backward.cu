@@ -14,10 +14,12 @@ constexpr uint32_t kColumnSlices = 37;  // widest rows: slices of the batch that
 
 inline __host__ __device__ uint32_t PartialPitch(uint32_t cols) { return (cols + 3U) / 4U * 4U; }
 
-// What a kernel is made of: packs of a thread, threads, rows on their way, CTAs an SM.
-template <class Tdy, class Tx, class Lay_, int kThreads_>
+// What a kernel is made of: packs of a thread, threads, rows on their way, CTAs an SM. kPair: a cluster of two CTAs has a row, half of
+// its columns each, and adds up the two sums of it through each other's shared memory.
+template <class Tdy, class Tx, class Lay_, int kThreads_, bool kPair_ = false>
 struct Form {
     using Lay = Lay_;
+    static constexpr bool kPair = kPair_;
     static constexpr int V = Lay::V, kThreads = kThreads_, E = Lay::E;
     static constexpr int kBytes = E * (sizeof(Tdy) + sizeof(Tx)) * kThreads;  // of a row of every group
     static constexpr int kDepth = V == 1 || kBytes > (32 << 10) ? 2 : kBytes >= (16 << 10) ? 3 : 6;
@@ -27,6 +29,23 @@ struct Form {
     static constexpr uint32_t kGammaBytes = E * kThreads * 4U;
 };
 
+// Adds the other CTA's sums of the row that the cluster is at, in the order of the CTAs. Two places take turns: who writes one again has
+// passed the barrier behind the other, and with it this CTA's reading of the first. (A CTA leaves after the barrier of its last row,
+// behind which nothing is written to it.)
+__device__ __forceinline__ void AddOther(float2& place, float (&s)[2]) {
+    const uint32_t rank = blockIdx.x & 1U;
+    if (threadIdx.x == 0U) {
+        uint32_t there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&place))), "r"(rank ^ 1U));
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(s[0]), "f"(s[1]) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const volatile float2& got = place;
+    const float2 other = make_float2(got.x, got.y);
+    s[0] = rank == 0U ? s[0] + other.x : other.x + s[0];
+    s[1] = rank == 0U ? s[1] + other.y : other.y + s[1];
+}
+
 template <class Tdy, class Tx, class Tdx, class F>
 __global__ void __launch_bounds__(F::kThreads, F::kCtas)
 BackwardKernel(const Backward a) {
@@ -35,15 +54,18 @@ BackwardKernel(const Backward a) {
     constexpr int V = F::V, E = F::E, D = F::kDepth, kThreads = F::kThreads, kPairs = Held<E>::kPairs;
     __shared__ float buffer[2 * 2 * (kThreads / 32)];
     Group g = MakeGroup(a.lanes, buffer);
-    const Share share = MakeShare(g, a.rows);
-    const Lay lay(g, a.cols);
-    typename F::RingDy ring_dy(a.dy, a.dy_pitch, a.rows, memory + F::kGammaBytes, share, lay);
-    typename F::RingX ring_x(a.x, a.x_pitch, a.rows, memory + F::kGammaBytes + F::RingDy::kBytes, share, lay);
+    const uint32_t cta = F::kPair ? blockIdx.x / 2U : blockIdx.x, ctas = F::kPair ? gridDim.x / 2U : gridDim.x;
+    const uint32_t half = ((a.cols - 1U) / V + 2U) / 2U * V, begin = F::kPair && (blockIdx.x & 1U) != 0U ? half : 0U;  // the first column, and how many
+    const Lay lay(g, !F::kPair ? a.cols : begin != 0U ? a.cols - half : half);
+    const Share share = MakeShare(g, a.rows, cta, ctas);
+    typename F::RingDy ring_dy(static_cast<const Tdy*>(a.dy) + begin, a.dy_pitch, a.rows, memory + F::kGammaBytes, share, lay);
+    typename F::RingX ring_x(static_cast<const Tx*>(a.x) + begin, a.x_pitch, a.rows, memory + F::kGammaBytes + F::RingDy::kBytes, share, lay);
     const float per_col = 1.0f / static_cast<float>(a.cols);
-    Tdx* dx = static_cast<Tdx*>(a.dx) + share.first * a.dx_pitch + lay.base;
+    Tdx* dx = static_cast<Tdx*>(a.dx) + share.first * a.dx_pitch + begin + lay.base;
     const uint64_t dx_step = share.stride * a.dx_pitch;
     ring_dy.Clear(lay);
     ring_x.Clear(lay);
+    if constexpr (F::kPair) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // (both are there to be written to)
     dependent_begin();
 #pragma unroll
     for (int d = 0; d < D; ++d) {
@@ -60,13 +82,14 @@ BackwardKernel(const Backward a) {
     load_statistics(0);
     float2* gamma_at = reinterpret_cast<float2*>(memory) + threadIdx.x;  // this thread's columns: in registers they would spill beside the sums
     Held<E> gy, xhat, sums[kSums];
-    LoadColumns(xhat, lay, a.gamma, 1.0f);
+    LoadColumns(xhat, lay, a.gamma != nullptr ? a.gamma + begin : nullptr, 1.0f);
 #pragma unroll
     for (int k = 0; k < kPairs; ++k) gamma_at[k * kThreads] = xhat.pair[k];
 #pragma unroll
     for (uint32_t n = 0; n < kSums; ++n)
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) sums[n].pair[k] = Both(0.0f);
+    __shared__ float2 pair_sums[2];
     uint32_t slot = 0;
     for (uint32_t t = 0; t < share.turns; ++t) {
         const bool in = t < share.mine;
@@ -88,6 +111,7 @@ BackwardKernel(const Backward a) {
         }
         float s[2] = {s1.x + s1.y, s2.x + s2.y};
         Reduce(g, s);
+        if constexpr (F::kPair) AddOther(pair_sums[t & 1U], s);
         if (V == 1) __syncwarp();  // (everybody has what it read of the slot: the sums needed it)
         ring_dy.Fetch(lay, slot, t + D < share.mine);
         ring_x.Fetch(lay, slot, t + D < share.mine);
@@ -111,11 +135,11 @@ BackwardKernel(const Backward a) {
     __syncthreads();  // (the rings are no longer read)
     // this CTA's column sums: the groups in order
     const uint32_t pitch = PartialPitch(a.cols);
-    float* partial = a.partial + static_cast<uint64_t>(blockIdx.x) * kSums * pitch;
+    float* partial = a.partial + static_cast<uint64_t>(cta) * kSums * pitch;
 #pragma unroll
     for (uint32_t k = 0; k < kSums; ++k) {
         if (a.sums[k] == nullptr) continue;
-        float* to = gridDim.x > 1U ? partial + k * pitch : a.sums[k];
+        float* to = (ctas > 1U ? partial + k * pitch : a.sums[k]) + begin;
         float* mine = g.count > 1U ? lanes_sums + g.index * a.cols : to;
 #pragma unroll
         for (int i = 0; i < Lay::NV; ++i)
@@ -253,20 +277,21 @@ template <class Tdy, class Tx, class Tdx, class F>
 mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint32_t groups = cut.threads / cut.lanes;
     const uint64_t want = (static_cast<uint64_t>(a.rows) + groups - 1U) / groups;
-    const uint32_t most = kSms * F::kCtas, ctas = static_cast<uint32_t>(want < most ? want : most);
+    const uint32_t most = kSms * F::kCtas / (F::kPair ? 2U : 1U), ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
     constexpr uint32_t smem = F::kGammaBytes + F::RingDy::kBytes + F::RingX::kBytes;
     static_assert(smem >= F::E * F::kThreads * 4U, "the sums of all groups, a float a column of each");
     static std::atomic<uint64_t> allowed{0};
     if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, F>, allowed, smem)) return MGT_CUDA_FAILURE;
-    Launch(BackwardKernel<Tdy, Tx, Tdx, F>, ctas, cut.threads, smem, on, a);
+    if constexpr (F::kPair) LaunchClusters(2U, BackwardKernel<Tdy, Tx, Tdx, F>, 2U * ctas, cut.threads, smem, on, a);
+    else Launch(BackwardKernel<Tdy, Tx, Tdx, F>, ctas, cut.threads, smem, on, a);
     ++*launches;
     if (ctas > 1U && (a.sums[0] != nullptr || a.sums[1] != nullptr || a.sums[2] != nullptr)) SumPartialRows(a, ctas, on, launches);
     return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
 }
 template <class Tdy, class Tx, class Tdx, int V>
 mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
-    const Cut cut = CutRow(a.rows, a.cols, V, kMostLanes);
+    Cut cut = CutRow(a.rows, a.cols, V, 2U * kMostLanes);
     if (cut.stream) {
         float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(a.cols));
         Launch(StreamMeansKernel<Tdy, Tx, V>, a.rows < 2U * kSms ? a.rows : 2U * kSms, 1024, 0, on, a, means);
@@ -279,6 +304,10 @@ mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
     }
     // (packs that a kernel has room for and the row does not have lie beyond its end)
     constexpr int kMost = kElements / V;
+    if (cut.threads > kMostLanes) {
+        cut.threads = cut.lanes = kMostLanes;  // of each of two CTAs
+        return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512, true>>(a, cut, on, launches);
+    }
     if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512>>(a, cut, on, launches);
     if constexpr (V == 1) {
         return SingleColumns(cut, [&](auto tag) { return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, typename decltype(tag)::type, 256>>(a, cut, on, launches); });
@@ -303,7 +332,7 @@ mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_
 }  // namespace
 
 uint64_t BackwardFloats(uint32_t rows, uint32_t cols) {
-    return static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(cols) + (cols > kElements * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
+    return static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(cols) + (cols > 2U * kElements * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
 }
 
 mgt_status_t LaunchBackward(Backward a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {

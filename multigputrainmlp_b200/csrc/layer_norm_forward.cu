@@ -32,9 +32,9 @@ ForwardKernel(const Forward a) {
     constexpr bool kFar = kThreads > 512;
     constexpr int V = Lay::V, E = Lay::E, D = kDepth<Tx, Lay, kThreads>, kPairs = Held<E>::kPairs;
     Group g = MakeGroup(a.lanes, buffer);
-    const Share share = MakeShare(g, a.rows);
+    const Share share = MakeShare(g, a.rows, blockIdx.x, gridDim.x);
     const Lay lay(g, a.cols);
-    Ring<Tx, Lay, kThreads, D> ring(a.x, a.x_pitch, a.rows, memory, share, lay);
+    Ring<Tx, Lay, kThreads, D> ring(static_cast<const Tx*>(a.x), a.x_pitch, a.rows, memory, share, lay);
     const float per_col = 1.0f / static_cast<float>(a.cols);
     Ty* y = static_cast<Ty*>(a.y) + share.first * a.y_pitch + lay.base;
     float* state = kTower ? a.state + share.first * a.x_pitch + lay.base : nullptr;
