@@ -16,7 +16,7 @@
 namespace {
 
 constexpr uint32_t kThreads = 256, kFinishThreads = 1024;
-constexpr int kUnroll = 4;  // 16-byte loads of a thread in flight
+constexpr uint32_t kUnroll = 4;  // 16-byte loads of a thread in flight
 constexpr uint32_t kLeastChunkBytes = 16384;  // four such loads a thread: more chunks than the chip holds CTAs, so that none waits long for a last one
 constexpr uint32_t kMostChunks = 4000;  // of whole length: longer chunks beyond, so that their sums fit into the shared memory of a CTA
 
@@ -69,23 +69,26 @@ __device__ __forceinline__ uint64_t HeadCount(const T* p, uint64_t n) {
 template <class T>
 __device__ double SumOfSquares(const T* p, uint64_t n) {
     const uint64_t head = HeadCount(p, n);
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    double s[2] = {0.0, 0.0};  // (four would not leave room for eight CTAs an SM)
     auto add = [&](float f, uint32_t j) {
         const double d = static_cast<double>(f);
-        s[j & 3U] = fma(d, d, s[j & 3U]);
+        s[j & 1U] = fma(d, d, s[j & 1U]);
     };
     if (threadIdx.x < head) add(Vec<T>::One(p[threadIdx.x]), 0);
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
     const uint32_t vectors = static_cast<uint32_t>((n - head) / Vec<T>::kCount);
-#pragma unroll kUnroll
-    for (uint32_t i = threadIdx.x; i < vectors; i += kThreads) {
-        const uint4 w = body[i];
+    for (uint32_t first = threadIdx.x; first < vectors; first += kUnroll * kThreads) {
+        uint4 w[kUnroll];
 #pragma unroll
-        for (uint32_t j = 0; j < Vec<T>::kCount; ++j) add(Vec<T>::Get(w, j), j);
+        for (uint32_t k = 0; k < kUnroll; ++k) w[k] = first + k * kThreads < vectors ? body[first + k * kThreads] : make_uint4(0U, 0U, 0U, 0U);
+#pragma unroll
+        for (uint32_t k = 0; k < kUnroll; ++k)
+#pragma unroll
+            for (uint32_t j = 0; j < Vec<T>::kCount; ++j) add(Vec<T>::Get(w[k], j), j);
     }
     const uint64_t at = head + vectors * Vec<T>::kCount + threadIdx.x;
     if (at < n) add(Vec<T>::One(p[at]), 0);
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    return s[0] + s[1];
 }
 
 template <class T>
@@ -100,12 +103,18 @@ __device__ void Scale(const T* p, T* out, uint64_t n, float scale, bool zero) {
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
     uint4* to = reinterpret_cast<uint4*>(out + head);
     const uint32_t vectors = static_cast<uint32_t>((n - head) / Vec<T>::kCount);
-#pragma unroll kUnroll
-    for (uint32_t i = threadIdx.x; i < vectors; i += kThreads) {
-        uint4 w = body[i];
+    for (uint32_t first = threadIdx.x; first < vectors; first += kUnroll * kThreads) {
+        uint4 w[kUnroll];
 #pragma unroll
-        for (uint32_t j = 0; j < Vec<T>::kCount; ++j) Vec<T>::Put(w, j, scaled(Vec<T>::Get(w, j)));
-        __stcs(to + i, w);
+        for (uint32_t k = 0; k < kUnroll; ++k)
+            if (first + k * kThreads < vectors) w[k] = body[first + k * kThreads];
+#pragma unroll
+        for (uint32_t k = 0; k < kUnroll; ++k) {
+            if (first + k * kThreads >= vectors) continue;
+#pragma unroll
+            for (uint32_t j = 0; j < Vec<T>::kCount; ++j) Vec<T>::Put(w[k], j, scaled(Vec<T>::Get(w[k], j)));
+            __stcs(to + first + k * kThreads, w[k]);
+        }
     }
     const uint64_t at = head + vectors * Vec<T>::kCount + threadIdx.x;
     if (at < n) out[at] = Vec<T>::To(scaled(Vec<T>::One(p[at])));
@@ -129,7 +138,7 @@ __device__ __forceinline__ double WarpSum(double s) {
 }
 
 template <uint32_t kMost>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 8)
 ChunkSquaresKernel(const __grid_constant__ Table<kMost> t, double* __restrict__ partial) {
     __shared__ double warps[kThreads / 32U];
     const uint32_t tensor = TensorOf(t, blockIdx.x);

@@ -158,8 +158,8 @@ BackwardKernel(const Backward a) {
     }
 }
 
-// sums[k][c] = the partial rows' values added up: 32 threads share four neighbouring columns, each adds every 32nd row in order (ten loads in
-// flight at most: one trip to L2), and the 32 then in order. Rows of partial sums are whole quads apart; what lies behind the last column is read and not used.
+// sums[k][c] = the partial rows' values added up: 32 threads share four neighbouring columns, each adds every 32nd row in order (ten at
+// most, all on their way at once), and the 32 then in order. Rows of partial sums are whole quads apart; what lies behind the last column is read and not used.
 constexpr uint32_t kSumQuads = 8, kSumParts = 32;
 __global__ void __launch_bounds__(kSumQuads * kSumParts)
 SumPartialRowsKernel(const Backward a, uint32_t rows, uint32_t pitch) {
@@ -172,10 +172,15 @@ SumPartialRowsKernel(const Backward a, uint32_t rows, uint32_t pitch) {
     if (quad * 4U < a.cols) {
         const float4* from = reinterpret_cast<const float4*>(a.partial + blockIdx.y * pitch) + quad;
         const uint64_t step = kSums * (pitch / 4U);
-#pragma unroll 10
-        for (uint32_t r = part; r < rows; r += kSumParts) {
-            const float4 v = from[r * step];
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        float4 v[(kMostCtas + kSumParts - 1U) / kSumParts];
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(v) / sizeof(v[0]); ++i) {
+            const uint32_t r = part + i * kSumParts;
+            v[i] = r < rows ? from[r * step] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(v) / sizeof(v[0]); ++i) {
+            s.x += v[i].x; s.y += v[i].y; s.z += v[i].z; s.w += v[i].w;
         }
     }
     part_sums[part][q] = s;
