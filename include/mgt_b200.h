@@ -259,7 +259,7 @@ mgt_status_t mgt_launch_float_to_half(const float* device_values, uint64_t count
  * may be dy or x, where type and pitch are the same; otherwise nothing overlaps. gamma NULL = ones, beta NULL = zeros;
  * mean and rstd (rows floats, the forward pass leaves them for the backward pass) may be NULL in the forward pass; dgamma, dbeta and
  * dbias may each be NULL (not wanted). gamma, beta and their gradients are fp32. A row with an infinity or a NaN gives NaN
- * in that row (and, in the backward pass, in the sums). Deviations from the mean are squared in fp32: up to 1e18.
+ * in that row (and, in the backward pass, in the sums). A row is added up in fp32 and deviations from its mean are squared there: up to 1e18.
  * The backward pass needs a workspace of mgt_layer_norm_backward_workspace_floats floats, 8-byte aligned (0 = invalid config); calls that may run at
  * the same time need one each. Everything lies on the current device. */
 enum { MGT_F32 = 0, MGT_F16 = 1, MGT_BF16 = 2 };
@@ -294,6 +294,7 @@ mgt_status_t mgt_launch_layer_norm_backward(const mgt_layer_norm_config_t* confi
  * A tensor is `count` elements side by side at `data` (any alignment of whole elements; count 0 is an empty tensor, whose norm is 0). The list is
  * read during the call and may then go; 1 to MGT_MAX_TENSORS tensors of MGT_MAX_TENSOR_ELEMENTS elements together. The workspace
  * (mgt_gradient_norm_workspace_floats floats, 8-byte aligned; 0 = invalid list) belongs to one call at a time.
+ * A tensor that is in the list twice counts twice. Where gradients are clipped, no two tensors that are written overlap.
  * mgt_launch_clip_gradients multiplies every element by the scale that device_result holds, in fp32, rounded once, in place or (out_tensors
  * not NULL: the same counts and types, not overlapping the list) to another place; a gradient whose norm is not finite becomes zero.
  * Everything lies on the current device. */

@@ -69,10 +69,11 @@ def _with_torch():
 def _address(t, type_code, elements, device):
     """The address behind a tensor that holds `elements` of a type from there on. Another type, another device than `device` (the host
     included) or too little behind the address raises _Unfit; None and plain addresses are the library's to judge."""
-    if t is None or isinstance(t, int):
+    try:
+        if t.dtype is not _DTYPES.get(type_code) or t.get_device() != device:
+            raise _Unfit
+    except AttributeError:  # no tensor
         return t
-    if t.dtype is not _DTYPES.get(type_code) or t.get_device() != device:
-        raise _Unfit
     if (t.numel() if t.is_contiguous() else t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()) < elements:
         raise _Unfit
     return t.data_ptr()

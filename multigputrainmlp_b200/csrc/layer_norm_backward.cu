@@ -298,7 +298,7 @@ template <class Tdy, class Tx, class Tdx, int V>
 mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
     Cut cut = CutRow(a.rows, a.cols, V, 2U * kMostLanes);
     if (cut.stream) {
-        float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(a.cols));
+        float2* means = reinterpret_cast<float2*>(a.partial + static_cast<uint64_t>(kColumnSlices) * kSums * PartialPitch(a.cols));
         Launch(StreamMeansKernel<Tdy, Tx, V>, a.rows < 2U * kSms ? a.rows : 2U * kSms, 1024, 0, on, a, means);
         const uint32_t slices = a.rows < kColumnSlices ? a.rows : kColumnSlices, rows_each = (a.rows - 1U) / slices + 1U;
         const uint32_t used = (a.rows - 1U) / rows_each + 1U;
@@ -337,7 +337,8 @@ mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_
 }  // namespace
 
 uint64_t BackwardFloats(uint32_t rows, uint32_t cols) {
-    return static_cast<uint64_t>(kMostCtas) * kSums * PartialPitch(cols) + (cols > 2U * kElements * kMostLanes ? 2ULL * rows : 0ULL) + 2ULL;
+    const bool stream = cols > 2U * kElements * kMostLanes;  // (from there on whatever the packs are)
+    return static_cast<uint64_t>(stream ? kColumnSlices : kMostCtas) * kSums * PartialPitch(cols) + (stream ? 2ULL * rows : 0ULL) + 4ULL;
 }
 
 mgt_status_t LaunchBackward(Backward a, int32_t dy_type, int32_t x_type, int32_t dx_type, LaunchOn on, uint32_t* launches) {

@@ -293,6 +293,36 @@ def test_same_results_every_time_on_any_stream_and_from_a_graph(rows, cols):
     assert all(torch.equal(p, q) for p, q in zip(other[:7], captured[:7]))
 
 
+def test_widest_rows():
+    rows, cols = 3, 1 << 20
+    values, gamma, beta, g = make(rows, cols, 12)
+    y, mean, rstd = torch.empty_like(values), torch.empty(rows, device=DEV), torch.empty(rows, device=DEV)
+    cfg = mgt.LayerNormConfig(rows, cols)
+    assert mgt.launch_layer_norm(cfg, values, gamma, beta, y, mean, rstd) == 0
+    check_forward(values, "f32", y, mean, rstd, gamma, beta)
+    dy = torch.randn(rows, cols, device=DEV, generator=g)
+    dx, sums = torch.empty_like(values), [torch.empty(cols, device=DEV) for _ in range(3)]
+    floats = mgt.layer_norm_backward_workspace_floats(cfg)
+    ws = torch.full((floats + 64,), MARK, device=DEV)
+    assert mgt.launch_layer_norm_backward(cfg, dy, values, gamma, mean, rstd, dx, *sums, ws, floats) == 0
+    check_backward(dy, values, gamma, mean, rstd, dx, "f32", sums)
+    assert (ws[floats:] == MARK).all()
+
+
+def test_workspace_that_begins_off_16_bytes():
+    rows, cols = 900, 222
+    values, gamma, _, g = make(rows, cols, 13)
+    dy = torch.randn(rows, cols, device=DEV, generator=g)
+    _, m, r, *_ = exact_forward(values, None, None)
+    cfg = mgt.LayerNormConfig(rows, cols)
+    floats = mgt.layer_norm_backward_workspace_floats(cfg)
+    ws = torch.full((floats + 66,), MARK, device=DEV)
+    dx, sums = torch.empty_like(values), [torch.empty(cols, device=DEV) for _ in range(3)]
+    assert mgt.launch_layer_norm_backward(cfg, dy, values, gamma, m.float(), r.float(), dx, *sums, ws[2:], floats) == 0
+    check_backward(dy, values, gamma, m.float(), r.float(), dx, "f32", sums)
+    assert (ws[floats + 2:] == MARK).all() and (ws[:2] == MARK).all()
+
+
 def test_rows_beyond_32_bit_offsets():
     rows, cols, pitch = 18, 300, 1 << 27  # the last row begins at element 17 * 2^27 > 2^31
     free, _ = torch.cuda.mem_get_info()
@@ -325,3 +355,4 @@ def test_tensors_that_do_not_fit_are_refused():
     assert run(mean=torch.zeros(9, device=DEV)) == 1 and run(x=x[:, :20].expand(10, 20)) == 0  # (a view of the same rows: enough lies behind it)
     assert run(x=torch.zeros(1, 1, device=DEV).expand(10, 40)) == 1
     assert run(mgt.LayerNormConfig(10, 40, x_pitch=41)) == 1
+    assert run(mgt.LayerNormConfig(10, 40, x_type=3)) == 1 and run(mgt.LayerNormConfig(10, 40, y_type=-1)) == 1

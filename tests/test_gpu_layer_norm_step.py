@@ -49,15 +49,15 @@ class Embedding(torch.autograd.Function):
     """Sums of rounded table rows; the table's gradient takes the rounded gradient."""
 
     @staticmethod
-    def forward(ctx, onehot, table, kind):
+    def forward(ctx, onehot, table, kind, table_kind):
         ctx.save_for_backward(onehot)
-        ctx.kind = kind
+        ctx.kind = kind if table_kind == "same" else table_kind
         return onehot @ rounded(table, kind)
 
     @staticmethod
     def backward(ctx, dy):
         (onehot,) = ctx.saved_tensors
-        return None, onehot.T @ rounded(dy, ctx.kind), None
+        return None, onehot.T @ rounded(dy, ctx.kind), None, None
 
 
 class RoundForward(torch.autograd.Function):
@@ -77,8 +77,8 @@ def layer_norm(z, gamma, beta, eps):
     return d / torch.sqrt((d * d).mean(1, keepdim=True) + eps) * gamma + beta
 
 
-def model(shape, w, states, labels, kind, ce=False, eps=1e-5):
-    """(loss, gradient) in 64 bits; kind: the operands' type, None for none."""
+def model(shape, w, states, labels, kind, ce=False, eps=1e-5, table_kind="same"):
+    """(loss, gradient) in 64 bits; kind: the operands' type, None for none; table_kind: what the gradient of the table is taken from."""
     w = torch.from_numpy(np.asarray(w, np.float32)).to(DEV).double().requires_grad_()
     n, h1, h2, r, out = states.shape[0], shape.hd1, shape.hd2, shape.residual_blocks, shape.output_dim
     at = [0]
@@ -96,7 +96,7 @@ def model(shape, w, states, labels, kind, ce=False, eps=1e-5):
     norms = [(take(h2), take(h2)) for _ in range(r + 1)]
     index = torch.from_numpy(states[:, :shape.state_len].astype(np.int64)).to(DEV) + torch.arange(shape.state_len, device=DEV) * shape.state_value_pad
     onehot = torch.zeros(n, rows, device=DEV, dtype=torch.float64).scatter_(1, index, 1.0)
-    a1 = torch.relu(Embedding.apply(onehot, table, kind) + RoundForward.apply(b_in, kind))
+    a1 = torch.relu(Embedding.apply(onehot, table, kind, table_kind) + RoundForward.apply(b_in, kind))
     x = torch.relu(layer_norm(Product.apply(a1, wh, kind) + bh, *norms[0], eps))
     for (w1, b1, w2, b2), (gamma, beta) in zip(blocks, norms[1:]):
         inner = torch.relu(Product.apply(x, w1, kind) + b1)
@@ -111,16 +111,16 @@ def model(shape, w, states, labels, kind, ce=False, eps=1e-5):
     return float(loss.detach()), w.grad.cpu().numpy()
 
 
-def run_engine(eng, shape, w, states, labels, *, callback=None, floats=None):
+def run_engine(eng, shape, w, states, labels, *, callback=None, half_table=True, **more):
     cshape = cshape_of(shape)
     b = states.shape[0]
     dw, ds = torch.from_numpy(w).to(DEV), torch.from_numpy(states).to(DEV)
     dl = torch.from_numpy(np.ascontiguousarray(labels)).to(DEV)
     loss, grad = torch.zeros(1, device=DEV), torch.full((w.size + 16,), float("nan"), device=DEV)
-    floats = mgt.mlp_loss_grad_workspace_floats(cshape, b, layer_norm=True) if floats is None else floats
+    floats = mgt.mlp_loss_grad_workspace_floats(cshape, b, 1, half_table, layer_norm=True)
     ws = torch.full((floats + 256,), float("nan"), device=DEV)
     ws[floats:] = 5.0
-    st = eng.launch_mlp_loss_grad(cshape, dw, None, ds, dl, b, loss, grad, ws, floats, gradient_ready=callback)
+    st = eng.launch_mlp_loss_grad(cshape, dw, None, ds, dl, b, loss, grad, ws, floats, gradient_ready=callback, use_half_input_grad=half_table, **more)
     assert st == 0, mgt.status_name(st)
     st, code = eng.check()
     assert st == 0, f"device status {code}"
@@ -178,6 +178,27 @@ def test_engine_with_layer_norm_matches_the_model(oracle, dims, n, bf16, ce, smo
     assert_close(shape, loss_g, grad_g, loss_m, grad_m, grad_exact, tol=8e-3 if bf16 else 1e-3)
     assert len(seen) == 2 * shape.residual_blocks + 4
     assert seen[-1] == (2 * shape.residual_blocks + 3, shape.param_count, 2 * (shape.residual_blocks + 1) * shape.hd2) and seen[-2][1] == 0
+
+
+def test_fp32_table_gradient_profile_and_early_range(oracle):
+    shape, w, states, labels = make_case(oracle, (72, 72, 96, 40, 2, 1), 333, seed=45)
+    loss_m, grad_m = model(shape, w, states, labels, torch.float16, table_kind=None)
+    _, grad_exact = model(shape, w, states, labels, None)
+    eng = mgt.Engine(0)
+    early = []
+    try:
+        assert eng.set_layer_norm(True) == 0
+        loss_g, grad_g = run_engine(eng, shape, w, states, labels, half_table=False)
+        assert_close(shape, loss_g, grad_g, loss_m, grad_m, grad_exact, tol=1e-3)
+        plain = run_engine(eng, shape, w, states, labels)
+        profile = mgt.BackwardProfile()
+        timed = run_engine(eng, shape, w, states, labels, profile=profile)
+        assert np.array_equal(plain[1], timed[1]) and profile.residual_forward_ms > 0
+        assert eng.set_early_range_hook(lambda u, i, off, cnt, s: early.append((off, cnt)) or 0) == 0
+        hooked = run_engine(eng, shape, w, states, labels)
+        assert np.array_equal(plain[1], hooked[1]) and early == [(0, 72 * 72 * 96 + 96)]
+    finally:
+        eng.close()
 
 
 def test_gradient_against_differences_of_the_loss(oracle):
@@ -351,6 +372,10 @@ def test_trainer_with_layer_norm_and_clipping(tmp_path, oracle):
     run_trainer(b, "--steps", 2, *common[:-2])
     assert np.array_equal(np.fromfile(a / "checkpoint" / "state.f32.bin", np.float32), np.fromfile(b / "checkpoint" / "state.f32.bin", np.float32))
     assert not os.path.exists(b / "grad_norm.jsonl")
+    # without a mirror of the weights, with the stages timed, without files
+    run_trainer(tmp_path / "other", "--steps", 2, *common, "--persistent-half-weights", 0, "--backward-profile", 1, "--write-artifacts", 0)
+    other = [json.loads(line)["grad_norm"] for line in open(tmp_path / "other" / "grad_norm.jsonl")]
+    assert other == [c["grad_norm"] for c in clips[:2]]  # (the mirror holds what the step rounds itself)
     for bad in (("--ln-eps", 0), ("--max-grad-norm", -1), ("--batch-norm", 1), ("--linear-fp16", 0)):
         assert run_trainer(tmp_path / "bad", "--steps", 1, *common, *bad, check=False).returncode != 0, bad
     # without the normalisation's checkpoint a run with it cannot be resumed

@@ -111,3 +111,15 @@ def test_gradient_norm_and_clip_arguments():
     cfg = mgt.AdamWKernelConfig(8, 1, 1e-3)
     adamw = lambda clip_at=0x4000, w=0x10000: mgt.launch_adamw_kernel_with_clip(cfg, w, None, 0x20000, clip_at, 0x30000, 0x40000, stream=0)  # noqa: E731
     assert adamw(clip_at=None) == 1 and adamw(clip_at=0x4002) == 1 and adamw(w=0x10004) == 1
+
+
+def test_workspace_of_layer_norm_never_shrinks_with_the_batch():
+    for dims, batches in (((72, 72, 333, 77, 3, 1), range(1, 40000, 401)), ((72, 72, 2560, 224, 16, 1), range(3500, 3800)), ((16, 16, 64, 512, 0, 2), range(1, 300))):
+        shape = mgt.CudaMlpShape(*dims)
+        for half_table in (True, False):
+            sizes = [mgt.mlp_loss_grad_workspace_floats(shape, b, 1, half_table, layer_norm=True) for b in batches]
+            assert sizes[0] > 0 and all(x <= y for x, y in zip(sizes, sizes[1:]))
+    shape = mgt.CudaMlpShape(16, 16, 64, 64, 1, 1)
+    assert mgt.mlp_loss_grad_workspace_floats(shape, 64, layer_norm=True, use_half_linear=False) == 0  # fp32 layers have no normalisation
+    assert mgt.mlp_loss_grad_workspace_floats(shape, 64, layer_norm=True, batch_norm=True) == 0
+    assert mgt.mlp_loss_grad_workspace_floats(shape, 0, layer_norm=True) == 0
