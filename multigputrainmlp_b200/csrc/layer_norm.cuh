@@ -297,10 +297,39 @@ __device__ __forceinline__ Pack<T, V> PackOf(const Held<E>& v, int i) {
 // A vector of columns that may begin anywhere; `none` for no vector, zero beyond the row's end.
 template <class Lay>
 __device__ __forceinline__ void LoadColumns(Held<Lay::E>& out, const Lay& lay, const float* p, float none) {
+    if (Lay::V > 1 && p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15U) == 0U) {  // (single loads of packs touch a sector a lane)
+#pragma unroll
+        for (int i = 0; i < Lay::NV; ++i)
+#pragma unroll
+            for (int j = 0; j < Lay::V; j += 4) {
+                const float4 v = lay.Has(i) ? *reinterpret_cast<const float4*>(p + lay.base + lay.Offset(i) + j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                out.pair[(i * Lay::V + j) / 2] = make_float2(v.x, v.y);
+                out.pair[(i * Lay::V + j) / 2 + 1] = make_float2(v.z, v.w);
+            }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < Lay::NV; ++i)
 #pragma unroll
         for (int j = 0; j < Lay::V; ++j) out.Set(i * Lay::V + j, lay.Has(i) ? (p != nullptr ? p[lay.base + lay.Offset(i) + j] : none) : 0.0f);
+}
+template <class Lay>
+__device__ __forceinline__ void StoreColumns(float* p, const Held<Lay::E>& v, const Lay& lay) {
+    if (Lay::V > 1 && (reinterpret_cast<uintptr_t>(p) & 15U) == 0U) {
+#pragma unroll
+        for (int i = 0; i < Lay::NV; ++i)
+#pragma unroll
+            for (int j = 0; j < Lay::V; j += 4) {
+                const float2 a = v.pair[(i * Lay::V + j) / 2], b = v.pair[(i * Lay::V + j) / 2 + 1];
+                if (lay.Has(i)) *reinterpret_cast<float4*>(p + lay.base + lay.Offset(i) + j) = make_float4(a.x, a.y, b.x, b.y);
+            }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < Lay::NV; ++i)
+#pragma unroll
+        for (int j = 0; j < Lay::V; ++j)
+            if (lay.Has(i)) p[lay.base + lay.Offset(i) + j] = v.Get(i * Lay::V + j);
 }
 template <int E>
 __device__ __forceinline__ float SumOf(const Held<E>& v) {

@@ -133,24 +133,28 @@ BackwardKernel(const Backward a) {
     CopiesWait<0>();
     float* lanes_sums = reinterpret_cast<float*>(memory);
     __syncthreads();  // (the rings are no longer read)
-    // this CTA's column sums: the groups in order
-    const uint32_t pitch = PartialPitch(a.cols);
+    // this CTA's column sums: the groups of a warp by shuffles, then the warps (or the groups of several) in order
+    for (uint32_t o = g.lanes; o < 32U; o <<= 1)
+#pragma unroll
+        for (uint32_t n = 0; n < kSums; ++n)
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                const float2 v = sums[n].pair[k];
+                sums[n].pair[k] = Add2(v, make_float2(__shfl_xor_sync(0xffffffffU, v.x, o), __shfl_xor_sync(0xffffffffU, v.y, o)));
+            }
+    const uint32_t pitch = PartialPitch(a.cols), teams = kThreads / max(g.lanes, 32U), team = threadIdx.x / max(g.lanes, 32U);
+    const bool speaks = g.lanes >= 32U || (threadIdx.x & 31U) < g.lanes;
     float* partial = a.partial + static_cast<uint64_t>(cta) * kSums * pitch;
 #pragma unroll
     for (uint32_t k = 0; k < kSums; ++k) {
         if (a.sums[k] == nullptr) continue;
         float* to = (ctas > 1U ? partial + k * pitch : a.sums[k]) + begin;
-        float* mine = g.count > 1U ? lanes_sums + g.index * a.cols : to;
-#pragma unroll
-        for (int i = 0; i < Lay::NV; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (lay.Has(i)) mine[lay.base + lay.Offset(i) + j] = sums[k].Get(i * V + j);
-        if (g.count > 1U) {
+        if (speaks) StoreColumns(teams > 1U ? lanes_sums + team * pitch : to, sums[k], lay);
+        if (teams > 1U) {
             __syncthreads();
             for (uint32_t c = threadIdx.x; c < a.cols; c += kThreads) {
                 float s = 0.0f;
-                for (uint32_t l = 0; l < g.count; ++l) s += lanes_sums[l * a.cols + c];
+                for (uint32_t l = 0; l < teams; ++l) s += lanes_sums[l * pitch + c];
                 to[c] = s;
             }
             __syncthreads();
@@ -285,7 +289,7 @@ mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint32_t most = kSms * F::kCtas / (F::kPair ? 2U : 1U), ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
     constexpr uint32_t smem = F::kGammaBytes + F::RingDy::kBytes + F::RingX::kBytes;
-    static_assert(smem >= F::E * F::kThreads * 4U, "the sums of all groups, a float a column of each");
+    static_assert(smem >= F::E * F::kThreads * 4U + F::kThreads / 8U * 4U, "the sums of all warps or groups, a float a column of each");
     static std::atomic<uint64_t> allowed{0};
     if (!AllowShared(BackwardKernel<Tdy, Tx, Tdx, F>, allowed, smem)) return MGT_CUDA_FAILURE;
     if constexpr (F::kPair) LaunchClusters(2U, BackwardKernel<Tdy, Tx, Tdx, F>, 2U * ctas, cut.threads, smem, on, a);
