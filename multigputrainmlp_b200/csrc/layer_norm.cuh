@@ -339,7 +339,7 @@ __device__ __forceinline__ float SumOf(const Held<E>& v) {
     return s.x + s.y;
 }
 // ---- host side: how a row is cut
-constexpr uint32_t kElements = 16;  // that a thread holds of a row at most
+constexpr uint32_t kElements = 16;  // that a thread holds of a row
 struct Cut {
     uint32_t nv;         // packs a thread
     uint32_t lanes, threads;
@@ -351,8 +351,8 @@ inline uint32_t PowerOfTwo(uint32_t n) {
     return p;
 }
 // As few lanes a row as can hold it, which makes the reductions short, or more where the rows are too few to fill the chip's threads.
-inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v, uint32_t most_lanes) {
-    const uint32_t packs = (cols - 1U) / v + 1U, most = kElements / v;
+inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v, uint32_t most_lanes, uint32_t elements = kElements) {
+    const uint32_t packs = (cols - 1U) / v + 1U, most = elements / v;
     Cut c{1, 1, 256, false};
     if (packs > most * most_lanes) {
         c.stream = true;

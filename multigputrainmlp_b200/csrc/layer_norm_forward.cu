@@ -18,18 +18,22 @@ __device__ __forceinline__ Moments Finish(float first, const float (&sums)[2], f
 }
 
 template <class Tx, class Lay, int kThreads>
-constexpr int kDepth = kThreads > 512 ? (sizeof(Tx) == 2 ? 2 : 1) : Lay::V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : Lay::E * sizeof(Tx) >= 64 ? 3 : Lay::E * sizeof(Tx) >= 32 ? 5 : 8;
+constexpr int kDepth = kThreads * Lay::E > 8192 ? (sizeof(Tx) == 2 ? 2 : 1) : Lay::V == 1 ? (sizeof(Tx) == 2 ? 4 : 3) : Lay::E > 16 ? 2 : Lay::E * sizeof(Tx) >= 64 ? 3 : Lay::E * sizeof(Tx) >= 32 ? 5 : 8;
+template <class Tx, class Lay, int kThreads>
+constexpr uint32_t kCtas = kThreads > 256 ? 1 : (Lay::V == 1 && Lay::E > 8) || Lay::E * sizeof(Tx) >= 128 ? 2 : 3;  // an SM (single columns take more registers, 32 fp32 values more shared memory)
+// Whether scale and shift lie in shared memory, for want of registers: rows of more than a warp's 512 columns, of which a thread holds 32, so
+// that fewer warps have to meet for a row.
 template <class Lay, int kThreads>
-constexpr uint32_t kCtas = kThreads > 256 ? 1 : Lay::V == 1 && Lay::E > 8 ? 2 : 3;  // an SM (single columns take more registers)
+constexpr bool kFarColumns = Lay::E > 16 || kThreads > 512;
 
 // kTower: x is a layer's output before its normalisation, the normalised row is added to the fp32 residual stream, and what a ReLU leaves
 // goes to the stream and, as the next product's operand, to y.
 template <class Tx, class Ty, class Lay, int kThreads, bool kTower>
-__global__ void __launch_bounds__(kThreads, kCtas<Lay, kThreads>)
+__global__ void __launch_bounds__(kThreads, kCtas<Tx, Lay, kThreads>)
 ForwardKernel(const Forward a) {
     extern __shared__ __align__(16) char memory[];  // the ring, then gamma and beta where registers have no room for them
     __shared__ float buffer[2 * 2 * (kThreads / 32)];
-    constexpr bool kFar = kThreads > 512;
+    constexpr bool kFar = kFarColumns<Lay, kThreads>;
     constexpr int V = Lay::V, E = Lay::E, D = kDepth<Tx, Lay, kThreads>, kPairs = Held<E>::kPairs;
     Group g = MakeGroup(a.lanes, buffer);
     const Share share = MakeShare(g, a.rows, blockIdx.x, gridDim.x);
@@ -47,14 +51,14 @@ ForwardKernel(const Forward a) {
         CopiesEnd();
     }
     Held<E> gamma, beta, v;
-    float2* far = reinterpret_cast<float2*>(memory + Ring<Tx, Lay, kThreads, D>::kBytes) + threadIdx.x;
+    float4* far = reinterpret_cast<float4*>(memory + Ring<Tx, Lay, kThreads, D>::kBytes) + g.lane;  // {two of gamma, two of beta} of a lane, for all groups
     if constexpr (kFar) {
-        LoadColumns(v, lay, a.gamma, 1.0f);
+        LoadColumns(gamma, lay, a.gamma, 1.0f);
+        LoadColumns(beta, lay, a.beta, 0.0f);
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) far[k * kThreads] = v.pair[k];
-        LoadColumns(v, lay, a.beta, 0.0f);
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) far[(kPairs + k) * kThreads] = v.pair[k];
+        for (int k = 0; k < kPairs; ++k)
+            if (g.index == 0U) far[k * g.lanes] = make_float4(gamma.pair[k].x, gamma.pair[k].y, beta.pair[k].x, beta.pair[k].y);
+        __syncthreads();
     } else {
         LoadColumns(gamma, lay, a.gamma, 1.0f);
         LoadColumns(beta, lay, a.beta, 0.0f);
@@ -97,8 +101,10 @@ ForwardKernel(const Forward a) {
             }
             const float2 rstd = Both(mo.rstd), off = Both(-mo.shift * mo.rstd);
 #pragma unroll
-            for (int k = 0; k < kPairs; ++k)
-                v.pair[k] = Fma2(Fma2(v.pair[k], rstd, off), kFar ? far[k * kThreads] : gamma.pair[k], kFar ? far[(kPairs + k) * kThreads] : beta.pair[k]);
+            for (int k = 0; k < kPairs; ++k) {
+                const float4 q = kFar ? far[k * g.lanes] : make_float4(gamma.pair[k].x, gamma.pair[k].y, beta.pair[k].x, beta.pair[k].y);
+                v.pair[k] = Fma2(Fma2(v.pair[k], rstd, off), make_float2(q.x, q.y), make_float2(q.z, q.w));
+            }
             lay.Each([&](int i, bool has) {
                 if (!has) return;
                 const uint32_t at = lay.Offset(i);
@@ -182,27 +188,35 @@ mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
     const uint64_t want = (static_cast<uint64_t>(a.rows) + rows - 1U) / rows;
     a.lanes = cut.lanes;
     static std::atomic<uint64_t> allowed{0};
-    constexpr uint32_t smem = Ring<Tx, Lay, kThreads, kDepth<Tx, Lay, kThreads>>::kBytes + (kThreads > 512 ? Lay::E * kThreads * 8U : 0U);
-    if (!AllowShared(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, allowed, smem)) return MGT_CUDA_FAILURE;
-    const uint32_t most = 148U * kCtas<Lay, kThreads>;
+    constexpr uint32_t ring = Ring<Tx, Lay, kThreads, kDepth<Tx, Lay, kThreads>>::kBytes, far = kFarColumns<Lay, kThreads> ? Lay::E * 8U : 0U;
+    if (!AllowShared(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, allowed, ring + far * kThreads)) return MGT_CUDA_FAILURE;
+    const uint32_t smem = ring + far * cut.lanes, most = 148U * kCtas<Tx, Lay, kThreads>;
     Launch(ForwardKernel<Tx, Ty, Lay, kThreads, kTower>, static_cast<uint32_t>(want < most ? want : most), cut.threads, smem, on, a);
     return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
 }
 // (packs that a kernel has room for and the row does not have lie beyond its end)
 template <class Tx, class Ty, int V, bool kTower>
 mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
-    const Cut cut = CutRow(a.rows, a.cols, V, 1024);
+    // more columns than a warp holds of 16 a lane: packs by 32 a lane
+    const bool wide = V > 1 && !kTower && a.cols > (sizeof(Tx) == 2 ? 32U : 512U) * kElements;
+    const Cut cut = wide ? CutRow(a.rows, a.cols, V, 512, 2U * kElements) : CutRow(a.rows, a.cols, V, 1024);
     constexpr int kMost = kElements / V;
     if (cut.stream || (kTower && cut.threads > 256U)) {
         if constexpr (kTower) return MGT_INVALID_CONFIG;  // (no tower is that wide)
         Launch(StreamForwardKernel<Tx, Ty, V>, a.rows < 296U ? a.rows : 296U, 1024, 0, on, a);
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
-    if constexpr (!kTower)
-        if (cut.threads > 256U) {
-            using Lay = Layout<V, kMost, 32, V == 1 ? 8 : 0>;
-            return cut.threads > 512U ? Run<Tx, Ty, Lay, 1024, false>(a, cut, on) : Run<Tx, Ty, Lay, 512, false>(a, cut, on);
-        }
+    if constexpr (V == 1 && !kTower) {
+        using Lay = Layout<1, kMost, 32, 8>;
+        if (cut.threads > 512U) return Run<Tx, Ty, Lay, 1024, false>(a, cut, on);
+        if (cut.threads > 256U) return Run<Tx, Ty, Lay, 512, false>(a, cut, on);
+    }
+    if constexpr (V > 1 && !kTower) {
+        using Lay = Layout<V, 2 * kMost, 32, 0>;
+        if (cut.threads > 256U) return wide ? Run<Tx, Ty, Lay, 512, false>(a, cut, on) : Run<Tx, Ty, Layout<V, kMost, 32, 0>, 512, false>(a, cut, on);
+        if constexpr (sizeof(Tx) == 2)
+            if (cut.nv > kMost) return Run<Tx, Ty, Lay, 256, false>(a, cut, on);
+    }
     if constexpr (V == 1) {
         return SingleColumns(cut, [&](auto tag) { return Run<Tx, Ty, typename decltype(tag)::type, 256, kTower>(a, cut, on); });
     } else {
