@@ -253,7 +253,7 @@ mgt_status_t mgt_launch_float_to_half(const float* device_values, uint64_t count
  *   x_type, y_type, dx_type  types of x, of y and dy, and of dx. A 16-bit x goes with y and dy of its own type or fp32; dx has the
  *                            type of x, or any where x and dy are fp32.
  *   x_pitch, y_pitch, dx_pitch  elements from row to row (0 = cols) of x, of y and dy, and of dx; not less than cols. Elements between
- *                            cols and the pitch are neither read nor written.
+ *                            cols and the pitch are not written, and what they hold does not matter.
  * cols 1 to MGT_LAYER_NORM_MAX_COLS; rows may be 0: nothing is read then, and the three sums are set to zero. Any alignment of whole
  * elements will do; rows that begin on 16 bytes (8 beside an fp32 operand for a 16-bit one) are moved in wider accesses. y may be x, and dx
  * may be dy or x, where type and pitch are the same; otherwise nothing overlaps. gamma NULL = ones, beta NULL = zeros;

@@ -1,6 +1,6 @@
-// Layer normalisation: how rows are held and fetched. A row of C columns is shared by `lanes` threads (a power of two, at most a CTA); thread
-// t has the packs t, t + lanes, ... of V neighbouring elements, 16 elements at most. Several rows lie side by side in a CTA. Groups
-// of up to 32 lanes reduce by shuffles, wider ones through shared memory and a barrier of their own.
+// Layer normalisation: how rows are held and fetched. A row of C columns is shared by `lanes` threads (a power of two, at most a CTA), which
+// hold 16 or 32 of its elements each. Several rows lie side by side in a CTA. Groups of up to 32 lanes reduce by shuffles, wider ones
+// through shared memory and a barrier of their own.
 //
 // The kernels are bound by HBM, and what that takes is bytes in flight: some 45 KB an SM at 6.5 TB/s and a loaded latency of 1 us. One
 // row ahead in registers leaves 24 KB in flight (131 072 x 512 bf16 forward 107 us); so a thread copies what it will need of its next rows to
@@ -159,8 +159,8 @@ __device__ __forceinline__ Share MakeShare(const Group& g, uint32_t rows, uint32
 // Which columns a thread has.
 //   V > 1   packs t, t + lanes, ... of V columns; a pack is whole: the row has all of it or nothing.
 //   V = 1   L (8 or 32) neighbouring lanes share a stretch of the row, one column to each in turn; stretches differ by a column at most. So
-//           places are constants, and only the last kMasked turns have to look at the stretch's end. (Asking at every turn took 518 instead
-//           of 230 instructions a row of 301.)
+//           places are constants, and only the last kMasked turns have to look at the stretch's end. (131 072 rows of 301 fp16, forward: 54 us,
+//           82 where every turn asks.)
 template <int V_, int NV_, int L_, int kMasked_>
 struct Layout {
     static constexpr int V = V_, NV = NV_, L = L_, E = V * NV, kMasked = kMasked_;
@@ -350,7 +350,9 @@ inline uint32_t PowerOfTwo(uint32_t n) {
     while (p < n) p <<= 1;
     return p;
 }
-// As few lanes a row as can hold it, which makes the reductions short, or more where the rows are too few to fill the chip's threads.
+// As few lanes a row as can hold it, which makes the reductions short, or more where the rows are too few to fill the chip's threads - far too
+// few for more than a warp, whose lanes need no barrier (us, as few and more: forward 1 000 x 64 fp32 2.4, 1.8, 64 x 4 096 bf16 4.0, 2.6, but
+// 2 000 x 224 fp32 to fp16 2.4, with two warps a row 3.7).
 inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v, uint32_t most_lanes, uint32_t elements = kElements) {
     const uint32_t packs = (cols - 1U) / v + 1U, most = elements / v;
     Cut c{1, 1, 256, false};
@@ -360,7 +362,7 @@ inline Cut CutRow(uint32_t rows, uint32_t cols, uint32_t v, uint32_t most_lanes,
     }
     c.lanes = PowerOfTwo((packs - 1U) / most + 1U);
     if (v == 1U && c.lanes != 8U) c.lanes = c.lanes < 8U ? 8U : c.lanes < 32U ? 32U : c.lanes;  // stretches of 8 or 32 lanes
-    while (c.lanes < 256U && c.lanes < packs && static_cast<uint64_t>(rows) * c.lanes < 148ULL * 512ULL) c.lanes <<= 1;
+    while (c.lanes < 256U && c.lanes < packs && static_cast<uint64_t>(rows) * c.lanes < 148ULL * (c.lanes < 32U ? 512ULL : 128ULL)) c.lanes <<= 1;
     c.nv = (packs - 1U) / c.lanes + 1U;
     if (c.lanes > c.threads) c.threads = c.lanes;
     return c;

@@ -197,7 +197,8 @@ mgt_status_t Run(Forward a, const Cut& cut, LaunchOn on) {
 // (packs that a kernel has room for and the row does not have lie beyond its end)
 template <class Tx, class Ty, int V, bool kTower>
 mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
-    // more columns than a warp holds of 16 a lane: packs by 32 a lane
+    // 32 elements a thread for 16-bit rows beyond a warp's 512 columns (us, with 16 and with 32: 40 000 x 600 bf16 39.8, 26.2; x 1 024 41.4, 29.4;
+    // 16 384 x 4 096 67.6, 54.2), for fp32 ones where 512 threads of 16 are too few (20 000 x 1 024 28.4, 29.0; 7 000 x 8 192 79.5, 92.3)
     const bool wide = V > 1 && !kTower && a.cols > (sizeof(Tx) == 2 ? 32U : 512U) * kElements;
     const Cut cut = wide ? CutRow(a.rows, a.cols, V, 512, 2U * kElements) : CutRow(a.rows, a.cols, V, 1024);
     constexpr int kMost = kElements / V;
@@ -213,7 +214,9 @@ mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
     }
     if constexpr (V > 1 && !kTower) {
         using Lay = Layout<V, 2 * kMost, 32, 0>;
-        if (cut.threads > 256U) return wide ? Run<Tx, Ty, Lay, 512, false>(a, cut, on) : Run<Tx, Ty, Layout<V, kMost, 32, 0>, 512, false>(a, cut, on);
+        if constexpr (sizeof(Tx) == 4)
+            if (cut.threads > 256U && !wide) return Run<Tx, Ty, Layout<V, kMost, 32, 0>, 512, false>(a, cut, on);
+        if (cut.threads > 256U) return Run<Tx, Ty, Lay, 512, false>(a, cut, on);
         if constexpr (sizeof(Tx) == 2)
             if (cut.nv > kMost) return Run<Tx, Ty, Lay, 256, false>(a, cut, on);
     }
