@@ -286,7 +286,10 @@ template <class Tdy, class Tx, class Tdx, class F>
 mgt_status_t Run(Backward a, const Cut& cut, LaunchOn on, uint32_t* launches) {
     const uint32_t groups = cut.threads / cut.lanes;
     const uint64_t want = (static_cast<uint64_t>(a.rows) + groups - 1U) / groups;
-    const uint32_t most = kSms * F::kCtas / (F::kPair ? 2U : 1U), ctas = static_cast<uint32_t>(want < most ? want : most);
+    // One CTA an SM where two would not have four rows each for every group: half as many partial rows (us, with two and one: 20 000 x 64 bf16
+    // 9.1, 7.9; 5 000 x 512 bf16 11.0, 9.3; 1 000 x 2 048 bf16 13.8, 10.7)
+    const uint32_t full = kSms * F::kCtas / (F::kPair ? 2U : 1U), most = want < 4ULL * full && full > kSms ? kSms : full;
+    const uint32_t ctas = static_cast<uint32_t>(want < most ? want : most);
     a.lanes = cut.lanes;
     constexpr uint32_t smem = F::kGammaBytes + F::RingDy::kBytes + F::RingX::kBytes;
     static_assert(smem >= F::E * F::kThreads * 4U + F::kThreads / 8U * 4U, "the sums of all warps or groups, a float a column of each");
