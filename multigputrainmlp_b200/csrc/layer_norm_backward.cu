@@ -39,6 +39,7 @@ __device__ __forceinline__ void AddOther(float2& place, float (&s)[2]) {
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&place))), "r"(rank ^ 1U));
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(s[0]), "f"(s[1]) : "memory");
     }
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     const volatile float2& got = place;
     const float2 other = make_float2(got.x, got.y);
@@ -65,7 +66,10 @@ BackwardKernel(const Backward a) {
     const uint64_t dx_step = share.stride * a.dx_pitch;
     ring_dy.Clear(lay);
     ring_x.Clear(lay);
-    if constexpr (F::kPair) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // (both are there to be written to)
+    if constexpr (F::kPair) {  // (both are there to be written to)
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    }
     dependent_begin();
 #pragma unroll
     for (int d = 0; d < D; ++d) {

@@ -79,6 +79,9 @@ def make(rows, cols, seed, offset=0.0):
 FORWARD_TYPES = [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")]
 SHAPES = [(1, 1), (5, 2), (1, 224), (64, 8), (3, 31), (33, 77), (129, 224), (257, 512), (1300, 224), (100, 513), (40, 1000), (9, 4096), (5, 4097), (700, 2048),
           (3, 8192), (3, 8193), (2, 16384), (301, 9000), (3, 16385), (40, 20000), (1, 16386)]
+# one of each layout: single columns by 8 and by 32 lanes, packs of four in 16 bits, whole warps of packs
+SHAPES += [(10000, 11), (10000, 27), (10000, 61), (10000, 125), (6000, 77), (2500, 131), (2500, 231), (2500, 301), (2500, 501), (3000, 100), (50, 1004), (5, 5004),
+           (3000, 512), (2000, 1024), (500, 2050)]
 
 
 @pytest.mark.parametrize("x_kind,y_kind", FORWARD_TYPES)
