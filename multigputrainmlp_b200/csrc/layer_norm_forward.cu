@@ -7,6 +7,10 @@ namespace {
 
 // Mean and spread of a row that lies in registers, in two reductions: the sum, then the sums of d = x - m and of d * d. The second sum
 // of d corrects the rounding of the first mean (a row of large, nearly equal values), so that x - mean = d - shift is exact to an ulp.
+// The mean that a caller gets takes the correction only where it is larger than the spread. Below, what corrects is worse than what it
+// corrects: x - m drops the same bits of m for all x of one binade, an error of up to 2^-25 of the spread that no averaging makes smaller,
+// where the first sum is off by its own rounding alone (16-bit rows are often added up exactly): 1 346 rows of 5 304 fp16 values were off by
+// 6.5e-6 of their means with the correction, and without it the means of none of 600 shapes are off by more than 2e-7.
 struct Moments {
     float mean, shift, rstd;
 };
@@ -14,7 +18,7 @@ __device__ __forceinline__ Moments Finish(float first, const float (&sums)[2], f
     const float shift = sums[0] * per_col;
     const float var = sums[1] * per_col - shift * shift, v = (var < 0.0f ? 0.0f : var) + eps;  // (a NaN stays one)
     const float r = rsqrtf(v);
-    return {first + shift, shift, r * fmaf(-0.5f * v * r, r, 1.5f)};  // one Newton step: to an ulp, at a tenth of a root's and a division's price
+    return {first * first <= v ? first : first + shift, shift, r * fmaf(-0.5f * v * r, r, 1.5f)};  // one Newton step: to an ulp, at a tenth of a root's and a division's price
 }
 
 template <class Tx, class Lay, int kThreads>

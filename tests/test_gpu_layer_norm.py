@@ -359,3 +359,17 @@ def test_tensors_that_do_not_fit_are_refused():
     assert run(x=torch.zeros(1, 1, device=DEV).expand(10, 40)) == 1
     assert run(mgt.LayerNormConfig(10, 40, x_pitch=41)) == 1
     assert run(mgt.LayerNormConfig(10, 40, x_type=3)) == 1 and run(mgt.LayerNormConfig(10, 40, y_type=-1)) == 1
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 376), (70, 77), (301, 224), (40, 512), (33, 600), (9, 2049), (1346, 5304), (5, 12000), (3, 20000), (2, 20001)])
+def test_means_far_below_the_spread_have_the_sums_precision(kind, rows, cols):
+    """Values of 1/32 up to 127/32: with up to 20001 of them every partial sum is a multiple of 1/32 below 2^24 / 32, so fp32 adds them up
+    exactly in any order, and the mean is off by the roundings of 1 / cols and of the product: 2 u, and their product."""
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    x = (torch.randint(-127, 128, (rows, cols), device=DEV, generator=g) / 32.0).to(TYPES[kind][1])
+    mean = torch.empty(rows, device=DEV)
+    assert mgt.launch_layer_norm(mgt.LayerNormConfig(rows, cols, EPS, TYPES[kind][0], TYPES[kind][0]), x, None, None, torch.empty_like(x), mean, None) == 0
+    want, var = x.double().mean(1), x.double().var(1, correction=0)
+    assert (want.square() < 0.5 * var).all()
+    assert ((mean.double() - want).abs() <= 2.001 * U * want.abs()).all()
