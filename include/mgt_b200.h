@@ -294,9 +294,10 @@ mgt_status_t mgt_launch_layer_norm_backward(const mgt_layer_norm_config_t* confi
  * A tensor is `count` elements side by side at `data` (any alignment of whole elements; count 0 is an empty tensor, whose norm is 0). The list is
  * read during the call and may then go; 1 to MGT_MAX_TENSORS tensors of MGT_MAX_TENSOR_ELEMENTS elements together. The workspace
  * (mgt_gradient_norm_workspace_floats floats, 8-byte aligned; 0 = invalid list) belongs to one call at a time.
- * A tensor that is in the list twice counts twice. Where gradients are clipped, no two tensors that are written overlap.
+ * A tensor that is in the list twice counts twice.
  * mgt_launch_clip_gradients multiplies every element by the scale that device_result holds, in fp32, rounded once, in place or (out_tensors
- * not NULL: the same counts and types, not overlapping the list) to another place; a gradient whose norm is not finite becomes zero.
+ * not NULL: the same counts and types) to another place; a gradient whose norm is not finite becomes zero. A tensor that is written overlaps
+ * no other tensor of either list (MGT_INVALID_CONFIG): a factor would be applied twice, or to half of a tensor.
  * Everything lies on the current device. */
 #define MGT_MAX_TENSORS 1024u
 #define MGT_MAX_TENSOR_ELEMENTS (1ull << 40)

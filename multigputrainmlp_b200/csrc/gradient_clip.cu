@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -228,6 +229,38 @@ bool ValidTensors(const mgt_tensor_t* tensors, uint32_t count) {
     }
     return total <= MGT_MAX_TENSOR_ELEMENTS;
 }
+// Whether what a call writes overlaps itself or what it reads of other tensors: CTAs would race for it, and a factor might be applied twice.
+// One pass where the tensors lie in order of their addresses, as the views of one buffer do.
+bool Clashing(const mgt_tensor_t* tensors, uint32_t count, const mgt_tensor_t* out) {
+    struct Span {
+        uintptr_t begin, end;
+        uint32_t index;
+    };
+    Span written[MGT_MAX_TENSORS];
+    auto span = [](const mgt_tensor_t& t, uint32_t i) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(t.data);
+        return Span{at, at + t.count * (t.type == MGT_F32 ? 4U : 2U), i};
+    };
+    uint32_t n = 0;
+    bool sorted = true;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (tensors[i].count == 0) continue;
+        written[n] = span(out != nullptr ? out[i] : tensors[i], i);
+        if (n != 0 && written[n].begin < written[n - 1U].begin) sorted = false;
+        ++n;
+    }
+    if (!sorted) std::sort(written, written + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    for (uint32_t k = 1; k < n; ++k)
+        if (written[k].begin < written[k - 1U].end) return true;
+    if (out == nullptr) return false;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (tensors[i].count == 0) continue;
+        const Span read = span(tensors[i], i);
+        const Span* w = std::lower_bound(written, written + n, read.begin, [](const Span& a, uintptr_t at) { return a.end <= at; });
+        if (w != written + n && w->begin < read.end && !(w->index == i && w->begin == read.begin)) return true;
+    }
+    return false;
+}
 uint64_t ChunkOf(const mgt_tensor_t* tensors, uint32_t count) {
     uint64_t total = 0;
     uint32_t bytes = 2;  // of the widest type
@@ -302,6 +335,7 @@ mgt_status_t mgt_launch_clip_gradients(const mgt_tensor_t* tensors, uint32_t ten
         for (uint32_t i = 0; i < tensor_count; ++i)
             if (out_tensors[i].count != tensors[i].count || out_tensors[i].type != tensors[i].type) return MGT_INVALID_CONFIG;
     }
+    if (Clashing(tensors, tensor_count, out_tensors)) return MGT_INVALID_CONFIG;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (tensor_count <= 96U) RunScale<96>(tensors, tensor_count, out_tensors, device_result, s);
     else RunScale<MGT_MAX_TENSORS>(tensors, tensor_count, out_tensors, device_result, s);

@@ -123,3 +123,20 @@ def test_workspace_of_layer_norm_never_shrinks_with_the_batch():
     assert mgt.mlp_loss_grad_workspace_floats(shape, 64, layer_norm=True, use_half_linear=False) == 0  # fp32 layers have no normalisation
     assert mgt.mlp_loss_grad_workspace_floats(shape, 64, layer_norm=True, batch_norm=True) == 0
     assert mgt.mlp_loss_grad_workspace_floats(shape, 0, layer_norm=True) == 0
+
+
+def test_clipping_refuses_tensors_that_share_memory():
+    """(On a machine with a GPU only the refusals are made: the addresses are no memory.)"""
+    lib = _lib.load()
+    clip = lambda rows, out=None: int(lib.mgt_launch_clip_gradients(  # noqa: E731
+        ctypes.cast(entries(*rows), ctypes.c_void_p), len(rows), 0x4000, ctypes.cast(entries(*out), ctypes.c_void_p) if out else None, None))
+    a, b, c = (0x1000, 10, 0), (0x1028, 8, 1), (0x1038, 8, 2)  # side by side: 40 bytes, 16, 16
+    for rows in ((a, a), (a, b, a), ((0x1024, 4, 0), a), (a, (0x1026, 1, 1)), (b, c, (0x1036, 1, 1)), (c, b, (0x1028, 4, 2)), (a, (None, 0, 0), (0x1000, 1, 0))):
+        assert clip(rows) == 1, rows
+    far = [(0x9000 + d - 0x1000, n, k) for d, n, k in (a, b, c)]
+    for out in ([far[0], far[0][:1] + (8, 1), far[2]], [(0x1004, 10, 0), far[1], far[2]], [(0x1038, 10, 0), far[1], far[2]], [far[0], (0x1000, 8, 1), far[2]],
+                [far[0], far[1], (0x1028, 8, 2)]):
+        assert clip((a, b, c), out) == 1, out
+    if not torch.cuda.is_available():  # what fits reaches the launch, which has no device here
+        assert clip((a, b, c)) == 4 and clip((c, a, b)) == 4 and clip((a, b, c), far) == 4 and clip((c, a, b), (c, a, b)) == 4
+        assert clip((a, (0x1000, 0, 0), b)) == 4 and clip((b, a), ((0xfe0, 8, 1), (0x1038, 10, 0))) == 4
