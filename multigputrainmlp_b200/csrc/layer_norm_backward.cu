@@ -22,7 +22,9 @@ struct Form {
     static constexpr bool kPair = kPair_;
     static constexpr int V = Lay::V, kThreads = kThreads_, E = Lay::E;
     static constexpr int kBytes = E * (sizeof(Tdy) + sizeof(Tx)) * kThreads;  // of a row of every group
-    static constexpr int kDepth = V == 1 || kBytes > (32 << 10) ? 2 : kBytes >= (16 << 10) ? 3 : 6;
+    // no more than it takes (us, with 2 and 3 of 16 KB and more: 53 248 x 224 fp32 29.7, 30.1; 20 000 x 1 024 46.5, 48.3; with 2, 3 and 6 of 12 KB: 100 000 x 384
+    // bf16 49.1, 49.2, 50.9)
+    static constexpr int kDepth = V == 1 || kBytes >= (12 << 10) ? 2 : 3;
     static constexpr int kCtas = kThreads > 256 ? 1 : 2;
     using RingDy = Ring<Tdy, Lay, kThreads, kDepth>;
     using RingX = Ring<Tx, Lay, kThreads, kDepth>;
@@ -324,12 +326,16 @@ mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
         cut.threads = cut.lanes = kMostLanes;  // of each of two CTAs
         return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512, true>>(a, cut, on, launches);
     }
+    if constexpr (V == 4)
+        if (cut.threads > 256U && cut.nv == 3) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, 3, 32, 0>, 512>>(a, cut, on, launches);
     if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512>>(a, cut, on, launches);
     if constexpr (V == 1) {
         return SingleColumns(cut, [&](auto tag) { return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, typename decltype(tag)::type, 256>>(a, cut, on, launches); });
     } else {
         constexpr int kFew = V == 4 ? 2 : 1;
         if (cut.nv <= kFew) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kFew, 32, 0>, 256>>(a, cut, on, launches);
+        if constexpr (V == 4)
+            if (cut.nv == 3) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, 3, 32, 0>, 256>>(a, cut, on, launches);
         return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, 0>, 256>>(a, cut, on, launches);
     }
 }
@@ -340,7 +346,10 @@ mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_
                RowsAligned(a.dx, a.dx_pitch, a.rows, dx_type, v);
     };
     if constexpr (sizeof(Tdy) == 2 && sizeof(Tx) == 2 && sizeof(Tdx) == 2)
-        if (whole(8)) return RunByWidth<Tdy, Tx, Tdx, 8>(a, on, launches);
+        if (whole(8)) {  // three packs of four columns where two of eight leave more places empty (us, as eights and as fours: 20 001 x 2 056 bf16 84.8, 79.8)
+            const Cut fours = CutRow(a.rows, a.cols, 4, 2U * kMostLanes);
+            if (fours.stream || fours.nv != 3 || fours.lanes > kMostLanes) return RunByWidth<Tdy, Tx, Tdx, 8>(a, on, launches);
+        }
     if (whole(4)) return RunByWidth<Tdy, Tx, Tdx, 4>(a, on, launches);
     return RunByWidth<Tdy, Tx, Tdx, 1>(a, on, launches);
 }

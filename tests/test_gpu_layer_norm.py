@@ -373,3 +373,19 @@ def test_means_far_below_the_spread_have_the_sums_precision(kind, rows, cols):
     want, var = x.double().mean(1), x.double().var(1, correction=0)
     assert (want.square() < 0.5 * var).all()
     assert ((mean.double() - want).abs() <= 2.001 * U * want.abs()).all()
+
+
+# rows whose threads hold three packs: of eight columns (1 to 512 lanes a row), of four (8 to 512 lanes); enough rows not to be spread further
+THREE_PACKS = [(75800, 24), (20001, 88), (9500, 160), (9500, 96), (4801, 304), (4740, 384), (600, 768), (299, 1280), (151, 2056), (150, 2560), (9, 6000), (7, 12000)]
+
+
+@pytest.mark.parametrize("x_kind,y_kind", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f32"), ("f32", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("rows,cols", THREE_PACKS)
+def test_forward_with_three_packs(rows, cols, x_kind, y_kind):
+    test_forward(rows, cols, x_kind, y_kind)
+
+
+@pytest.mark.parametrize("dy_kind,x_kind,dx_kind", [("f16", "f16", "f16"), ("bf16", "bf16", "bf16"), ("f32", "f32", "f32"), ("f32", "f32", "bf16"), ("f16", "f32", "f32")])
+@pytest.mark.parametrize("rows,cols", THREE_PACKS)
+def test_backward_with_three_packs(rows, cols, dy_kind, x_kind, dx_kind):
+    test_backward(rows, cols, dy_kind, x_kind, dx_kind)
