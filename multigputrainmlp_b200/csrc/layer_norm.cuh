@@ -384,7 +384,8 @@ inline mgt_status_t SingleColumns(const Cut& cut, F run) {
     if (cut.nv <= 4U) return run(Tag<Layout<1, 4, 32, 2>>{});
     if (cut.nv <= 6U) return run(Tag<Layout<1, 6, 32, 2>>{});
     if (cut.nv <= 8U) return run(Tag<Layout<1, 8, 32, 2>>{});
-    if (cut.nv <= 12U) return run(Tag<Layout<1, 12, 32, 4>>{});
+    if (cut.nv <= 10U) return run(Tag<Layout<1, 10, 32, 2>>{});
+    if (cut.nv <= 12U) return run(Tag<Layout<1, 12, 32, 2>>{});
     return run(Tag<Layout<1, 16, 32, 4>>{});
 }
 // Dynamic shared memory beyond 48 KB is an attribute of a kernel on a device: set on the first launch there.

@@ -322,13 +322,23 @@ mgt_status_t RunByWidth(const Backward& a, LaunchOn on, uint32_t* launches) {
     }
     // (packs that a kernel has room for and the row does not have lie beyond its end)
     constexpr int kMost = kElements / V;
+    // twelve columns a thread where they do (us, with sixteen and with twelve: 8 000 x 5 001 fp32 157, 98; 4 000 x 10 001 bf16 148, 124; 4 000 x 9 000 bf16
+    // 109, 100); rows of a 512-thread CTA by two CTAs of half as many columns a thread are slower (7 000 x 8 192 bf16 77.5, 147)
     if (cut.threads > kMostLanes) {
         cut.threads = cut.lanes = kMostLanes;  // of each of two CTAs
-        return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512, true>>(a, cut, on, launches);
+        if constexpr (V == 4)
+            if (cut.nv == 3) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, 3, 32, 0>, 512, true>>(a, cut, on, launches);
+        if constexpr (V == 1)
+            if (cut.nv <= 12U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<1, 12, 32, 4>, 512, true>>(a, cut, on, launches);
+        return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 4 : 0>, 512, true>>(a, cut, on, launches);
     }
-    if constexpr (V == 4)
-        if (cut.threads > 256U && cut.nv == 3) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, 3, 32, 0>, 512>>(a, cut, on, launches);
-    if (cut.threads > 256U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 8 : 0>, 512>>(a, cut, on, launches);
+    if (cut.threads > 256U) {
+        if constexpr (V == 4)
+            if (cut.nv == 3) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, 3, 32, 0>, 512>>(a, cut, on, launches);
+        if constexpr (V == 1)
+            if (cut.nv <= 12U) return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<1, 12, 32, 4>, 512>>(a, cut, on, launches);
+        return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, Layout<V, kMost, 32, V == 1 ? 4 : 0>, 512>>(a, cut, on, launches);
+    }
     if constexpr (V == 1) {
         return SingleColumns(cut, [&](auto tag) { return Run<Tdy, Tx, Tdx, Form<Tdy, Tx, typename decltype(tag)::type, 256>>(a, cut, on, launches); });
     } else {
@@ -348,7 +358,7 @@ mgt_status_t RunTyped(const Backward& a, int32_t dy_type, int32_t x_type, int32_
     if constexpr (sizeof(Tdy) == 2 && sizeof(Tx) == 2 && sizeof(Tdx) == 2)
         if (whole(8)) {  // three packs of four columns where two of eight leave more places empty (us, as eights and as fours: 20 001 x 2 056 bf16 84.8, 79.8)
             const Cut fours = CutRow(a.rows, a.cols, 4, 2U * kMostLanes);
-            if (fours.stream || fours.nv != 3 || fours.lanes > kMostLanes) return RunByWidth<Tdy, Tx, Tdx, 8>(a, on, launches);
+            if (fours.stream || fours.nv != 3) return RunByWidth<Tdy, Tx, Tdx, 8>(a, on, launches);
         }
     if (whole(4)) return RunByWidth<Tdy, Tx, Tdx, 4>(a, on, launches);
     return RunByWidth<Tdy, Tx, Tdx, 1>(a, on, launches);

@@ -223,9 +223,10 @@ mgt_status_t RunByWidth(const Forward& a, LaunchOn on) {
         return cudaGetLastError() == cudaSuccess ? MGT_OK : MGT_CUDA_FAILURE;
     }
     if constexpr (V == 1 && !kTower) {
-        using Lay = Layout<1, kMost, 32, 8>;
-        if (cut.threads > 512U) return Run<Tx, Ty, Lay, 1024, false>(a, cut, on);
-        if (cut.threads > 256U) return Run<Tx, Ty, Lay, 512, false>(a, cut, on);
+        using Less = Layout<1, 12, 32, 4>;  // (nine columns a thread at least; us, with 16 and with 12: 4 000 x 10 001 bf16 88.6, 81.7)
+        using Most = Layout<1, 16, 32, 4>;
+        if (cut.threads > 512U) return cut.nv <= 12U ? Run<Tx, Ty, Less, 1024, false>(a, cut, on) : Run<Tx, Ty, Most, 1024, false>(a, cut, on);
+        if (cut.threads > 256U) return cut.nv <= 12U ? Run<Tx, Ty, Less, 512, false>(a, cut, on) : Run<Tx, Ty, Most, 512, false>(a, cut, on);
     }
     if constexpr (V > 1 && !kTower) {
         using Lay = Layout<V, 2 * kMost, 32, 0>;

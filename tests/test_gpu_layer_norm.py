@@ -389,3 +389,14 @@ def test_forward_with_three_packs(rows, cols, x_kind, y_kind):
 @pytest.mark.parametrize("rows,cols", THREE_PACKS)
 def test_backward_with_three_packs(rows, cols, dy_kind, x_kind, dx_kind):
     test_backward(rows, cols, dy_kind, x_kind, dx_kind)
+
+
+# single columns, 9 to 16 a thread, in CTAs of 256, 512 and 1024 threads (or two of 512), at the ends of what each layout holds
+SINGLE = [(150, 2049), (150, 2559), (9, 4097), (9, 6143), (9, 6145), (9, 8191), (7, 8193), (7, 12287), (7, 12289), (7, 16383), (5000, 289), (5000, 319)]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", SINGLE)
+def test_single_columns_of_wide_rows(rows, cols, kind):
+    test_forward(rows, cols, kind, kind)
+    test_backward(rows, cols, kind, kind, kind)
