@@ -167,9 +167,10 @@ FinishNormKernel(const __grid_constant__ Table<kMost> t, const double* __restric
     __shared__ double chunks[kMostChunks + kMost], squares[kMost], warps[kFinishThreads / 32U];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31U, all = t.first_chunk[t.tensors];
     mgt::dependent_begin();
+    const double* sums = mgt::after_begin(partial);
 #pragma unroll
     for (uint32_t c = threadIdx.x; c < kMostChunks + kMost; c += kFinishThreads)
-        if (c < all) chunks[c] = partial[c];
+        if (c < all) chunks[c] = sums[c];
     __syncthreads();
     for (uint32_t k = warp; k < t.tensors; k += kFinishThreads / 32U) {
         const uint32_t end = t.first_chunk[k + 1U];
@@ -208,7 +209,8 @@ ScaleKernel(const __grid_constant__ Table<kMost> t, const __grid_constant__ Outp
     const uint64_t n = all - begin < t.chunk ? all - begin : t.chunk;
     const int32_t type = static_cast<int32_t>(t.count[tensor] >> kTypeShift);
     mgt::dependent_begin();
-    const float norm = result[0], scale = result[1];
+    const float* found = mgt::after_begin(result);
+    const float norm = found[0], scale = found[1];
     const bool zero = !(norm <= 3.402823466e38f);
     if (in_place && !zero && scale == 1.0f) return;  // every product is the value that is there
     if (type == MGT_F32) Scale(static_cast<const float*>(t.data[tensor]) + begin, static_cast<float*>(out.data[tensor]) + begin, n, scale, zero);
