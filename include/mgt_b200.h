@@ -171,7 +171,9 @@ uint64_t mgt_bn_param_count(const mgt_mlp_shape_t* shape); /* 2 * (residual_bloc
  *   device_exchange_buffer is where the engine puts those numbers - e.g. the buffer of a second, small mgt_comm (one
  *   communicator is driven from one stream: the gradient exchange keeps its own). Both NULL: statistics of this rank only.
  *   device_running_stats, if not NULL: (residual_blocks + 1) x {mean[hd2], var[hd2]}, updated every launch as
- *   running = (1 - momentum) * running + momentum * batch (variance unbiased over world_size * sample_count samples). */
+ *   running = (1 - momentum) * running + momentum * batch (variance unbiased over world_size * sample_count samples).
+ *   That is the forward pass, before any gradient is known: a caller who leaves a step out (mgt_launch_adamw_with_clip does where
+ *   the norm is not finite) keeps a copy of them and puts it back, as the trainer does. */
 typedef mgt_status_t (*mgt_stats_exchange_fn)(void* user, float* device_buffer, uint64_t float_count, void* stream);
 mgt_status_t mgt_engine_set_batch_norm_state(mgt_engine_t* engine, float* device_running_stats, float momentum,
                                              uint32_t world_size, float* device_exchange_buffer,
@@ -236,7 +238,7 @@ mgt_status_t mgt_launch_adamw_with_half_mirror(const mgt_adamw_config_t* config,
                                                float* device_m, float* device_v, void* stream);
 /* The same update of a gradient scaled by device_clip[1] (rounded to fp32), where mgt_launch_gradient_norm left {norm, scale} in device_clip: the gradient
  * itself stays as it is. A scale of 1 gives the plain update bit for bit. Where the norm is not finite, weights, mirror and moments stay as
- * they are. device_weights_half may be NULL (no mirror). No counterpart in the reference. */
+ * they are (running statistics of a batch normalisation are not its business: mgt_engine_set_batch_norm_state). device_weights_half may be NULL (no mirror). No counterpart in the reference. */
 mgt_status_t mgt_launch_adamw_with_clip(const mgt_adamw_config_t* config, float* device_weights, uint16_t* device_weights_half, const float* device_grad,
                                         const float* device_clip, float* device_m, float* device_v, void* stream);
 /* Replaces FloatToHalfMirrorKernel (native/tools/mgt_native_train_smoke.cu:68-72). */

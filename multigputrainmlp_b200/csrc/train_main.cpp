@@ -318,10 +318,12 @@ int main(int argc, char** argv) {
     const mgt_tensor_t whole_gradient{d_grad, T, MGT_F32, 0};
     const uint64_t norm_floats = clipped ? mgt_gradient_norm_workspace_floats(&whole_gradient, 1) : 0;
     float *d_clip = nullptr, *d_norm_ws = nullptr;  // {norm, scale} of a step, scratch
+    float* d_bn_kept = nullptr;  // the running statistics before a step that may be skipped: its forward pass has moved them by then
     if (ws_floats == 0 || d_grad == nullptr) return EXIT_FAILURE;
     cudaStream_t compute = nullptr, comm_stream = nullptr;
     bool ok = CUDA_OK(cudaMalloc(&d_w, T * 4)) && (!(opt.linear_fp16 && opt.persistent_half_weights) || CUDA_OK(cudaMalloc(&d_w_half, T * 2))) &&
               (!opt.batch_norm || CUDA_OK(cudaMalloc(&d_bn_running, NBN * 4))) &&
+              (!(clipped && opt.batch_norm) || CUDA_OK(cudaMalloc(&d_bn_kept, NBN * 4))) &&
               (!clipped || (CUDA_OK(cudaMalloc(&d_clip, 8)) && CUDA_OK(cudaMalloc(&d_norm_ws, norm_floats * 4)))) &&
               CUDA_OK(cudaMalloc(&d_labels, static_cast<uint64_t>(B) * opt.output_dim * 4)) &&
               (opt.output_dim == 1 || CUDA_OK(cudaMalloc(&d_walk_labels, static_cast<uint64_t>(B) * 4))) && CUDA_OK(cudaMalloc(&d_loss, 4)) &&
@@ -414,6 +416,7 @@ int main(int argc, char** argv) {
             exchange.average_only = clipped;
         }
         if (mgt_engine_set_early_range_hook(engine, overlap ? OnEarlyRange : nullptr, overlap ? &exchange : nullptr) != MGT_OK) return EXIT_FAILURE;
+        if (d_bn_kept != nullptr && !CUDA_OK(cudaMemcpyAsync(d_bn_kept, d_bn_running, NBN * 4, cudaMemcpyDeviceToDevice, compute))) return EXIT_FAILURE;
         mgt_backward_profile_t bw{};
         const mgt_status_t st = mgt_launch_mlp_loss_grad(engine, &shape, d_w, d_w_half, d_states, d_labels, B, d_loss, d_grad, d_ws, ws_floats,
                                                          opt.input_grad_partial_chunks, opt.input_grad_positions_per_block, opt.input_grad_fp16,
@@ -482,6 +485,9 @@ int main(int argc, char** argv) {
             if (finite) std::snprintf(row, sizeof(row), "{\"step\": %u, \"grad_norm\": %.9g, \"scale\": %.9g}\n", step, clip[0], clip[1]);
             else std::snprintf(row, sizeof(row), "{\"step\": %u, \"grad_norm\": null, \"scale\": 0}\n", step);
             grad_norms << row;
+            // a skipped step leaves the running statistics as they were, too (they may hold NaN for good otherwise)
+            if (!finite && d_bn_kept != nullptr && (!CUDA_OK(cudaMemcpyAsync(d_bn_running, d_bn_kept, NBN * 4, cudaMemcpyDeviceToDevice, compute)) ||
+                                                    !CUDA_OK(cudaStreamSynchronize(compute)))) return EXIT_FAILURE;
         }
         const uint32_t done = step + 1U;
         if (opt.checkpoint_period_steps != 0 && done % opt.checkpoint_period_steps == 0 && done != first_step + opt.steps) {
@@ -501,7 +507,7 @@ int main(int argc, char** argv) {
     for (cudaEvent_t ev : {ev_start, ev_walk, ev_backward, ev_allreduce, ev_stop, ev_comm_done, ev_early_done}) cudaEventDestroy(ev);
     for (void* p : {static_cast<void*>(d_target), static_cast<void*>(d_moves), static_cast<void*>(d_meta), static_cast<void*>(d_states), static_cast<void*>(d_v),
                     static_cast<void*>(d_m), static_cast<void*>(d_ws), static_cast<void*>(d_loss), static_cast<void*>(d_labels), static_cast<void*>(d_walk_labels),
-                    static_cast<void*>(d_w_half), static_cast<void*>(d_w), static_cast<void*>(d_bn_running), static_cast<void*>(d_clip), static_cast<void*>(d_norm_ws)})
+                    static_cast<void*>(d_w_half), static_cast<void*>(d_w), static_cast<void*>(d_bn_running), static_cast<void*>(d_bn_kept), static_cast<void*>(d_clip), static_cast<void*>(d_norm_ws)})
         if (p != nullptr) cudaFree(p);
     cudaStreamDestroy(comm_stream);
     cudaStreamDestroy(compute);
