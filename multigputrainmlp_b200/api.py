@@ -67,16 +67,46 @@ def _with_torch():
 
 
 def _address(t, type_code, elements, device):
-    """The address behind a tensor that holds `elements` of a type from there on. Another type, another device than `device` (the host
-    included) or too little behind the address raises _Unfit; None and plain addresses are the library's to judge."""
+    """The address behind a dense tensor that holds `elements` of a type. Another type, another device than `device` (the host
+    included), too few elements, or some that do not lie side by side, raise _Unfit; None and plain addresses are the library's to judge."""
     try:
         if t.dtype is not _DTYPES.get(type_code) or t.get_device() != device:
             raise _Unfit
     except AttributeError:  # no tensor
         return t
-    if (t.numel() if t.is_contiguous() else t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()) < elements:
+    if not t.is_contiguous() or t.numel() < elements:
         raise _Unfit
     return t.data_ptr()
+
+
+def _rows_address(t, type_code, elements, device, rows):
+    """The same for rows = (rows, columns, pitch), which may be a view too: of rows that lie so far apart."""
+    try:
+        if t.dtype is not _DTYPES.get(type_code) or t.get_device() != device:
+            raise _Unfit
+    except AttributeError:
+        return t
+    if t.is_contiguous():
+        if t.numel() < elements:
+            raise _Unfit
+    elif not _lies_in_rows(t, *rows) or t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < elements:
+        raise _Unfit
+    return t.data_ptr()
+
+
+def _lies_in_rows(t, rows, cols, pitch):
+    """Whether a view's last dimension lies side by side and the ones before it, taken together, are `rows` rows `pitch` apart, or more."""
+    dims = [(n, step) for n, step in zip(t.shape, t.stride()) if n != 1]
+    if cols == 1 and dims[-1][1] != 1:  # (a column of a matrix)
+        dims.append((1, 1))
+    if dims[-1][1] != 1:
+        return False
+    have = 1
+    for n, step in reversed(dims[:-1]):
+        if step != pitch * have:
+            return False
+        have *= n
+    return have >= rows
 
 
 def _raw_stream(stream, device):
@@ -366,7 +396,7 @@ def launch_float_to_half(device_values, count, device_half, stream=None) -> int:
 def launch_adamw_kernel_with_clip(config, device_weights, device_weights_half, device_grad, device_clip, device_m, device_v, stream=None) -> int:
     """mgt_launch_adamw_with_clip: the update of a gradient scaled by device_clip[1], skipped where the norm device_clip[0] is not finite
     (what launch_gradient_norm leaves). device_weights_half may be None. A tensor of another type, on another device than the
-    current one, or too small, is refused (1)."""
+    current one, too small, or not dense, is refused (1)."""
     n, d = config.param_count, _current_device(stream)
     try:
         w, half = _address(device_weights, F32, n, d), _address(device_weights_half, F16, n, d)
@@ -394,8 +424,10 @@ class LayerNormConfig:
         dx_type = self.x_type if self.dx_type is None else self.dx_type
         # (what a field would wrap around is refused as a config without columns)
         c = _LayerNorm(self.rows, self.cols, self.eps, self.x_type, self.y_type, dx_type, self.x_pitch, self.y_pitch, self.dx_pitch) if fits else _LayerNorm()
-        extents = tuple((self.rows - 1) * (pitch or self.cols) + self.cols if self.rows else 0 for pitch in (self.x_pitch, self.y_pitch, self.dx_pitch))
-        for name, value in (("_c", c), ("_reference", C.byref(c)), ("_extents", extents), ("_dx_type", dx_type)):
+        pitches = [pitch or self.cols for pitch in (self.x_pitch, self.y_pitch, self.dx_pitch)]
+        extents = tuple((self.rows - 1) * pitch + self.cols if self.rows else 0 for pitch in pitches)
+        layouts = tuple((self.rows, self.cols, pitch) for pitch in pitches)
+        for name, value in (("_c", c), ("_reference", C.byref(c)), ("_extents", extents + layouts), ("_dx_type", dx_type)):
             object.__setattr__(self, name, value)
 
     def c(self):
@@ -408,12 +440,13 @@ def validate_layer_norm_config(config: LayerNormConfig) -> int:
 
 def launch_layer_norm(config: LayerNormConfig, x, gamma, beta, y, mean=None, rstd=None, stream=None) -> int:
     """mgt_launch_layer_norm: y = gamma * (x - mean) * rstd + beta over the columns of every row; gamma, beta, mean and rstd may be None.
-    A tensor of another type, on another device than the current one, or too small, is refused (1)."""
+    A tensor of another type, on another device than the current one, or too small, is refused (1), and so are one that is not dense and, for x
+    and y, a view whose rows do not lie as the config says."""
     d = _current_device(stream)
-    x_extent, y_extent, _ = config._extents
+    x_extent, y_extent, _, x_rows, y_rows, _ = config._extents
     rows, cols = config.rows, config.cols
     try:
-        x, y = _address(x, config.x_type, x_extent, d), _address(y, config.y_type, y_extent, d)
+        x, y = _rows_address(x, config.x_type, x_extent, d, x_rows), _rows_address(y, config.y_type, y_extent, d, y_rows)
         gamma, beta, mean, rstd = _address(gamma, F32, cols, d), _address(beta, F32, cols, d), _address(mean, F32, rows, d), _address(rstd, F32, rows, d)
     except _Unfit:
         return 1
@@ -425,12 +458,13 @@ def layer_norm_backward_workspace_floats(config: LayerNormConfig) -> int:
 
 
 def launch_layer_norm_backward(config: LayerNormConfig, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, dbias, workspace, workspace_floats, stream=None) -> int:
-    """mgt_launch_layer_norm_backward: dx, and the sums over the rows dgamma, dbeta and dbias (each may be None)."""
+    """mgt_launch_layer_norm_backward: dx, and the sums over the rows dgamma, dbeta and dbias (each may be None). Tensors as above."""
     d = _current_device(stream)
-    x_extent, dy_extent, dx_extent = config._extents
+    x_extent, dy_extent, dx_extent, x_rows, dy_rows, dx_rows = config._extents
     rows, cols = config.rows, config.cols
     try:
-        dy, x, dx = _address(dy, config.y_type, dy_extent, d), _address(x, config.x_type, x_extent, d), _address(dx, config._dx_type, dx_extent, d)
+        dy, x = _rows_address(dy, config.y_type, dy_extent, d, dy_rows), _rows_address(x, config.x_type, x_extent, d, x_rows)
+        dx = _rows_address(dx, config._dx_type, dx_extent, d, dx_rows)
         gamma, mean, rstd = _address(gamma, F32, cols, d), _address(mean, F32, rows, d), _address(rstd, F32, rows, d)
         dgamma, dbeta, dbias = _address(dgamma, F32, cols, d), _address(dbeta, F32, cols, d), _address(dbias, F32, cols, d)
         workspace = _address(workspace, F32, workspace_floats, d)
