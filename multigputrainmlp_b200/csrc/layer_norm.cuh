@@ -182,6 +182,11 @@ struct Layout {
         if constexpr (V > 1) return base + Offset(i) < cols;
         else return i < NV - kMasked || (mask >> i & 1U) != 0U;
     }
+    // The values for the pair k of a thread's elements, zeros beyond the row's end.
+    __device__ __forceinline__ float2 HasPair(int k, float2 v) const {
+        if constexpr (V > 1) return Has(k / (V / 2)) ? v : make_float2(0.0f, 0.0f);
+        else return make_float2(Has(2 * k) ? v.x : 0.0f, Has(2 * k + 1) ? v.y : 0.0f);
+    }
     template <class F>
     __device__ __forceinline__ void Each(F f) const {  // f(i, whether the row has pack i)
 #pragma unroll

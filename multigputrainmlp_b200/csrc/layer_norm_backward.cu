@@ -107,8 +107,8 @@ BackwardKernel(const Backward a) {
         ring_x.Read(xhat, lay, slot, in);
         float2 s1 = Both(0.0f), s2 = Both(0.0f);
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {  // (beyond the row's end dy is zero, and with it all that xhat enters)
-            xhat.pair[k] = Mul2(Add2(xhat.pair[k], less), rstd);
+        for (int k = 0; k < kPairs; ++k) {  // (beyond the row's end dy is zero, and with it all that xhat enters: so that has to be a number)
+            xhat.pair[k] = Mul2(Add2(xhat.pair[k], lay.HasPair(k, less)), rstd);
             sums[0].pair[k] = Fma2(gy.pair[k], xhat.pair[k], sums[0].pair[k]);
             sums[1].pair[k] = Add2(gy.pair[k], sums[1].pair[k]);
             gy.pair[k] = Mul2(gy.pair[k], gamma_at[k * kThreads]);
