@@ -17,6 +17,8 @@
 #include <filesystem>
 #include <fstream>
 #include <iostream>
+#include <iterator>
+#include <string>
 #include <vector>
 
 using namespace mgt::host;
@@ -198,9 +200,15 @@ bool WriteLayerNormState(const std::string& dir, std::initializer_list<const std
         << ",\n  \"layer_layout\": \"layer 0 = hidden layer, layer k+1 = residual block k; gamma[width], beta[width]\"\n}\n";
     return static_cast<bool>(data) && static_cast<bool>(man);
 }
-bool ReadLayerNormState(const std::string& checkpoint_dir, std::vector<float>* scale_shift, std::vector<float>* m, std::vector<float>* v) {
-    std::ifstream data(checkpoint_dir + "/layer_norm.f32.bin", std::ios::binary);
-    if (!data) return false;
+// The state of the same model only: a file of that size, and a description, where there is one, of as many layers of that width.
+bool ReadLayerNormState(const std::string& checkpoint_dir, std::vector<float>* scale_shift, std::vector<float>* m, std::vector<float>* v, uint32_t layers, uint32_t width) {
+    std::ifstream data(checkpoint_dir + "/layer_norm.f32.bin", std::ios::binary | std::ios::ate);
+    if (!data || static_cast<uint64_t>(data.tellg()) != 3ULL * scale_shift->size() * sizeof(float)) return false;
+    std::ifstream man(checkpoint_dir + "/layer_norm.json");
+    const std::string text((std::istreambuf_iterator<char>(man)), std::istreambuf_iterator<char>());
+    auto says = [&](const char* key, uint32_t value) { return text.find("\"" + std::string(key) + "\": " + std::to_string(value) + ",") != std::string::npos; };
+    if (man.is_open() && (!says("layers", layers) || !says("width", width))) return false;
+    data.seekg(0);
     for (std::vector<float>* section : {scale_shift, m, v})
         data.read(reinterpret_cast<char*>(section->data()), static_cast<std::streamsize>(section->size() * sizeof(float)));
     return static_cast<bool>(data);
@@ -251,8 +259,8 @@ int main(int argc, char** argv) {
     InitialWeights(&weights);
     const bool resumed = !opt.resume_checkpoint.empty();
     if (resumed && !ReadCheckpoint(opt.resume_checkpoint, &weights, &adam_m, &adam_v)) return EXIT_FAILURE;
-    if (resumed && opt.layer_norm && !ReadLayerNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v)) {
-        std::cerr << "--layer-norm 1: " << opt.resume_checkpoint << "/layer_norm.f32.bin not found or too short\n";
+    if (resumed && opt.layer_norm && !ReadLayerNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v, opt.nrd + 1U, shape.hd2)) {
+        std::cerr << "--layer-norm 1: " << opt.resume_checkpoint << "/layer_norm.f32.bin not found, or of another model\n";
         return EXIT_FAILURE;
     }
     if (resumed && opt.batch_norm && !ReadBatchNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v, &bn_running)) {
