@@ -200,6 +200,15 @@ bool WriteLayerNormState(const std::string& dir, std::initializer_list<const std
         << ",\n  \"layer_layout\": \"layer 0 = hidden layer, layer k+1 = residual block k; gamma[width], beta[width]\"\n}\n";
     return static_cast<bool>(data) && static_cast<bool>(man);
 }
+// Files of a normalisation that a run does not have, left in its folder by one that had it: they are no part of what is written there now.
+bool RemoveNormState(const std::string& dir, const char* name) {
+    std::error_code error;
+    for (const char* end : {".f32.bin", ".json"}) {
+        std::filesystem::remove(dir + "/" + name + end, error);
+        if (error) return false;
+    }
+    return true;
+}
 // The state of the same model only: a file of that size, and a description, where there is one, of as many layers of that width.
 bool ReadLayerNormState(const std::string& checkpoint_dir, std::vector<float>* scale_shift, std::vector<float>* m, std::vector<float>* v, uint32_t layers, uint32_t width) {
     std::ifstream data(checkpoint_dir + "/layer_norm.f32.bin", std::ios::binary | std::ios::ate);
@@ -387,10 +396,13 @@ int main(int argc, char** argv) {
             std::vector<float> exported = weights;
             if (opt.batch_norm && mgt_fold_batch_norm(&shape, exported.data(), bn_scale_shift.data(), bn_running.data(), opt.bn_eps) != MGT_OK) return false;
             if (!WriteWeights(opt.output_dir, plan, exported)) return false;
-            if (opt.layer_norm && !WriteLayerNormState(opt.output_dir + "/weights", {&bn_scale_shift}, opt.nrd + 1U, shape.hd2, opt.ln_eps)) return false;
+            if (opt.layer_norm ? !WriteLayerNormState(opt.output_dir + "/weights", {&bn_scale_shift}, opt.nrd + 1U, shape.hd2, opt.ln_eps)
+                               : !RemoveNormState(opt.output_dir + "/weights", "layer_norm")) return false;
         }
         if (!WriteCheckpoint(opt.output_dir, plan, weights, adam_m, adam_v)) return false;
-        if (opt.layer_norm && !WriteLayerNormState(opt.output_dir + "/checkpoint", {&bn_scale_shift, &bn_m, &bn_v}, opt.nrd + 1U, shape.hd2, opt.ln_eps)) return false;
+        if (opt.layer_norm ? !WriteLayerNormState(opt.output_dir + "/checkpoint", {&bn_scale_shift, &bn_m, &bn_v}, opt.nrd + 1U, shape.hd2, opt.ln_eps)
+                           : !RemoveNormState(opt.output_dir + "/checkpoint", "layer_norm")) return false;
+        if (!opt.batch_norm && !RemoveNormState(opt.output_dir + "/checkpoint", "batch_norm")) return false;
         if (opt.batch_norm && !WriteBatchNormState(opt.output_dir, bn_scale_shift, bn_m, bn_v, bn_running, opt.nrd + 1U, shape.hd2, opt.bn_eps, opt.bn_momentum)) return false;
         std::ofstream out(opt.output_dir + "/checkpoint/step.txt", std::ios::trunc);
         out << steps_done << "\n";

@@ -47,3 +47,18 @@ def test_state_of_another_model_is_refused(tmp_path):
         assert train(tmp_path / "larger", "--layer-norm", 1, **size).returncode == 0
         (own / "layer_norm.f32.bin").write_bytes((tmp_path / "larger" / "checkpoint" / "layer_norm.f32.bin").read_bytes())
         assert train(tmp_path / "wrong", *resume).returncode != 0, size
+
+
+def names(folder):
+    return sorted(n for n in os.listdir(folder) if "norm" in n)
+
+
+def test_a_folder_holds_the_state_of_its_last_run_only(tmp_path):
+    d = tmp_path / "run"
+    layer, batch = ["layer_norm.f32.bin", "layer_norm.json"], ["batch_norm.f32.bin", "batch_norm.json"]
+    for flags, in_checkpoint, in_weights in ((["--layer-norm", 1], layer, layer), (["--batch-norm", 1], batch, []), (["--layer-norm", 1], layer, layer), ([], [], []),
+                                             (["--batch-norm", 1], batch, []), ([], [], [])):
+        assert train(d, *flags).returncode == 0
+        assert names(d / "checkpoint") == in_checkpoint and names(d / "weights") == in_weights, flags
+    for flag in ("--layer-norm", "--batch-norm"):  # the plain run's checkpoint is no checkpoint of either
+        assert train(tmp_path / "next", flag, 1, "--resume-checkpoint", d / "checkpoint").returncode != 0
