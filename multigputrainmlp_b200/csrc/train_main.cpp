@@ -268,6 +268,10 @@ int main(int argc, char** argv) {
     InitialWeights(&weights);
     const bool resumed = !opt.resume_checkpoint.empty();
     if (resumed && !ReadCheckpoint(opt.resume_checkpoint, &weights, &adam_m, &adam_v)) return EXIT_FAILURE;
+    if (resumed && !opt.layer_norm && std::filesystem::exists(opt.resume_checkpoint + "/layer_norm.f32.bin")) {
+        std::cerr << opt.resume_checkpoint << "/layer_norm.f32.bin: a model with layer normalisation, to be resumed with --layer-norm 1\n";
+        return EXIT_FAILURE;
+    }
     if (resumed && opt.layer_norm && !ReadLayerNormState(opt.resume_checkpoint, &bn_scale_shift, &bn_m, &bn_v, opt.nrd + 1U, shape.hd2)) {
         std::cerr << "--layer-norm 1: " << opt.resume_checkpoint << "/layer_norm.f32.bin not found, or of another model\n";
         return EXIT_FAILURE;

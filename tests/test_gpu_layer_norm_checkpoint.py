@@ -62,3 +62,12 @@ def test_a_folder_holds_the_state_of_its_last_run_only(tmp_path):
         assert names(d / "checkpoint") == in_checkpoint and names(d / "weights") == in_weights, flags
     for flag in ("--layer-norm", "--batch-norm"):  # the plain run's checkpoint is no checkpoint of either
         assert train(tmp_path / "next", flag, 1, "--resume-checkpoint", d / "checkpoint").returncode != 0
+
+
+def test_a_model_with_layer_norm_is_not_resumed_without(tmp_path):
+    assert train(tmp_path / "own", "--layer-norm", 1).returncode == 0
+    kept = (tmp_path / "own" / "checkpoint" / "state.f32.bin").read_bytes()
+    for flags in ([], ["--batch-norm", 1], ["--layer-norm", 0], ["--linear-fp16", 0]):
+        res = train(tmp_path / "own", "--resume-checkpoint", tmp_path / "own" / "checkpoint", *flags)
+        assert res.returncode != 0 and "--layer-norm 1" in res.stderr, flags
+    assert (tmp_path / "own" / "checkpoint" / "state.f32.bin").read_bytes() == kept
