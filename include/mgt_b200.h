@@ -300,7 +300,7 @@ mgt_status_t mgt_launch_layer_norm_backward(const mgt_layer_norm_config_t* confi
  * A tensor that is in the list twice counts twice.
  * mgt_launch_clip_gradients multiplies every element by the scale that device_result holds, in fp32, rounded once, in place or (out_tensors
  * not NULL: the same counts and types) to another place; a gradient whose norm is not finite becomes zero. A tensor that is written overlaps
- * no other tensor of either list (MGT_INVALID_CONFIG): a factor would be applied twice, or to half of a tensor.
+ * neither another one of either list nor device_result (MGT_INVALID_CONFIG): a factor would be applied twice, or to half of a tensor.
  * Everything lies on the current device. */
 #define MGT_MAX_TENSORS 1024u
 #define MGT_MAX_TENSOR_ELEMENTS (1ull << 40)

@@ -514,7 +514,7 @@ def launch_gradient_norm(tensors: TensorList, max_norm: float, result, tensor_no
 
 def launch_clip_gradients(tensors: TensorList, result, out_tensors: TensorList | None = None, stream=None) -> int:
     """mgt_launch_clip_gradients: every element times result[1], in place or into out_tensors (same counts and types). What is written
-    overlaps no other tensor of either list (status 1)."""
+    overlaps neither another tensor of either list nor result (status 1)."""
     d = _current_device(stream)
     if tensors.device != d or (out_tensors is not None and (out_tensors.device != d or out_tensors.count != tensors.count)):
         return 1

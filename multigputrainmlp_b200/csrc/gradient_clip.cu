@@ -231,9 +231,9 @@ bool ValidTensors(const mgt_tensor_t* tensors, uint32_t count) {
     }
     return total <= MGT_MAX_TENSOR_ELEMENTS;
 }
-// Whether what a call writes overlaps itself or what it reads of other tensors: CTAs would race for it, and a factor might be applied twice.
-// One pass where the tensors lie in order of their addresses, as the views of one buffer do.
-bool Clashing(const mgt_tensor_t* tensors, uint32_t count, const mgt_tensor_t* out) {
+// Whether what a call writes overlaps itself, what it reads of other tensors, or the factor: CTAs would race for it, and a factor might be
+// applied twice. One pass where the tensors lie in order of their addresses, as the views of one buffer do.
+bool Clashing(const mgt_tensor_t* tensors, uint32_t count, const float* result, const mgt_tensor_t* out) {
     struct Span {
         uintptr_t begin, end;
         uint32_t index;
@@ -254,11 +254,15 @@ bool Clashing(const mgt_tensor_t* tensors, uint32_t count, const mgt_tensor_t* o
     if (!sorted) std::sort(written, written + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
     for (uint32_t k = 1; k < n; ++k)
         if (written[k].begin < written[k - 1U].end) return true;
+    auto first_behind = [&](uintptr_t at) { return std::lower_bound(written, written + n, at, [](const Span& a, uintptr_t p) { return a.end <= p; }); };
+    const uintptr_t factor = reinterpret_cast<uintptr_t>(result);
+    const Span* over = first_behind(factor);
+    if (over != written + n && over->begin < factor + 2U * sizeof(float)) return true;
     if (out == nullptr) return false;
     for (uint32_t i = 0; i < count; ++i) {
         if (tensors[i].count == 0) continue;
         const Span read = span(tensors[i], i);
-        const Span* w = std::lower_bound(written, written + n, read.begin, [](const Span& a, uintptr_t at) { return a.end <= at; });
+        const Span* w = first_behind(read.begin);
         if (w != written + n && w->begin < read.end && !(w->index == i && w->begin == read.begin)) return true;
     }
     return false;
@@ -337,7 +341,7 @@ mgt_status_t mgt_launch_clip_gradients(const mgt_tensor_t* tensors, uint32_t ten
         for (uint32_t i = 0; i < tensor_count; ++i)
             if (out_tensors[i].count != tensors[i].count || out_tensors[i].type != tensors[i].type) return MGT_INVALID_CONFIG;
     }
-    if (Clashing(tensors, tensor_count, out_tensors)) return MGT_INVALID_CONFIG;
+    if (Clashing(tensors, tensor_count, device_result, out_tensors)) return MGT_INVALID_CONFIG;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (tensor_count <= 96U) RunScale<96>(tensors, tensor_count, out_tensors, device_result, s);
     else RunScale<MGT_MAX_TENSORS>(tensors, tensor_count, out_tensors, device_result, s);
