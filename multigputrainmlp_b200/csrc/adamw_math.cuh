@@ -60,7 +60,7 @@ __device__ __forceinline__ float AdamWUpdateOne(const AdamWScalars& s, float wei
     // fourth smallest rounds back to it): numerators of the slow path, for hundreds of steps or for good (15.5 M parameters of which a
     // seventh are such: 86 to 95 us instead of 76). The update is at most lr * |m| / bias1 / eps: where 2^27 times that is below the
     // weight, it is less than half of what separates the weight from its neighbours, which stays what it is whatever the quotient. So
-    // asked, all moments cost the same: 78 us, 74 from where bias1 is 1.
+    // asked, all moments cost the same: 80 us, 76 from where bias1 is 1.
     const bool still = fabsf(next_m) * s.still < fabsf(weight) && next_v >= 0.0f;  // (a second moment without a root makes a NaN of the weight)
     const float m_hat = s.bias1 == 1.0f ? next_m : DivByPositiveExact(next_m, s.bias1, still);  // (one from step 165 on with a beta1 of 0.9)
     const float v_hat = DivByPositiveExact(next_v, s.bias2);

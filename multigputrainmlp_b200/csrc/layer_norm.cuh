@@ -4,7 +4,7 @@
 //
 // The kernels are bound by HBM, and what that takes is bytes in flight: some 45 KB an SM at 6.5 TB/s and a loaded latency of 1 us. One
 // row ahead in registers leaves 24 KB in flight (131 072 x 512 bf16 forward 107 us); so a thread copies what it will need of its next rows to
-// shared memory asynchronously, two to four rows deep.
+// shared memory asynchronously, two to four rows deep (one, where a row of 32 KB and more fills a CTA).
 #pragma once
 
 #include "layer_norm.hpp"
