@@ -476,7 +476,8 @@ def launch_layer_norm_backward(config: LayerNormConfig, dy, x, gamma, mean, rstd
 
 class TensorList:
     """An array of mgt_tensor_t for the gradient-norm calls, and the tensors it stands for: float32, float16 or bfloat16, each dense,
-    all on one CUDA device. Built once where gradients stay in place; holds the tensors, not their values."""
+    all on one CUDA device. Built once where gradients stay in place: it stands for the memory that they have then, and holds that, whatever
+    becomes of a tensor (another `.data`, say) later. Not for memory that is taken away behind it (`untyped_storage().resize_`)."""
 
     def __init__(self, tensors):
         _with_torch()
@@ -492,6 +493,7 @@ class TensorList:
             devices.add(t.get_device())
         if len(devices) != 1:
             raise MgtError(1, "TensorList: tensors of one device")
+        self._memory = [t.untyped_storage() for t in self.tensors]
         self.device = devices.pop()
         self.pointer = C.addressof(self._array)
 
