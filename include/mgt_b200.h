@@ -262,7 +262,8 @@ mgt_status_t mgt_launch_float_to_half(const float* device_values, uint64_t count
  * mean and rstd (rows floats, the forward pass leaves them for the backward pass) may be NULL in the forward pass; dgamma, dbeta and
  * dbias may each be NULL (not wanted). gamma, beta and their gradients are fp32. A row with an infinity or a NaN gives NaN
  * in that row (and, in the backward pass, in the sums). A row is added up in fp32 and deviations from its mean are squared there: up to
- * 1e18 at any width, far beyond which a row gives NaN, too.
+ * 1e18 at any width (and values up to 1e22, whose mean is off by less than that), far beyond which a row gives NaN, too, and down to 1e-17 (to any with
+ * an eps of 1e-34 and more).
  * The backward pass needs a workspace of mgt_layer_norm_backward_workspace_floats floats, 8-byte aligned (0 = invalid config); calls that may run at
  * the same time need one each. Everything lies on the current device. */
 enum { MGT_F32 = 0, MGT_F16 = 1, MGT_BF16 = 2 };

@@ -46,3 +46,17 @@ def test_backward(rows, cols, kind):
     dx, sums = torch.empty_like(x), [torch.empty(cols, device=DEV) for _ in range(3)]
     assert mgt.launch_layer_norm_backward(cfg, dy, x, gamma, mean, rstd, dx, *sums, torch.empty(floats, device=DEV), floats) == 0
     check_backward(dy, x, gamma, mean, rstd, dx, kind, sums)
+
+
+@pytest.mark.parametrize("cols", [3, 77, 224, 600, 2049, 9000, 20000, 1 << 20])
+def test_large_values_without_large_deviations_are_finite(cols):
+    # the mean of values of 1e22 is off by (16 + 10 + cols / 1024) * 2^-24 of them at most, 6e17 for the widest rows: so the squares hold, and what the
+    # sums find is the row's spread and those roundings
+    x = torch.where(torch.arange(6, device=DEV)[:, None] % 2 == 0, 1e22, -7e21) * torch.ones(6, cols, device=DEV)
+    x[4:] *= 1 + 2.0 ** -20 * torch.randn(2, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(cols))
+    y, mean, rstd = torch.empty_like(x), torch.empty(6, device=DEV), torch.empty(6, device=DEV)
+    assert mgt.launch_layer_norm(mgt.LayerNormConfig(6, cols), x, None, None, y, mean, rstd) == 0
+    k = (64 + cols / 1024) * 2.0 ** -24
+    m = x.double().mean(1)
+    assert ((mean.double() - m).abs() <= k * x.double().abs().amax(1)).all()
+    assert torch.isfinite(y).all() and torch.isfinite(rstd).all() and (rstd > 0).all()
